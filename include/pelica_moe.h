@@ -358,6 +358,108 @@ PM_API int32_t pm_dequant(pm_ctx *ctx, int32_t ggml_type, const uint8_t *blocks,
 PM_API int32_t pm_quant_act(pm_ctx *ctx, int32_t mode, const float *x, size_t n, int8_t *q,
                             float *scale, int32_t *bsum);
 
+/* ---- tokens sorted by expert and back, and their gradients ------------------
+ * No counterpart in the reference: for hosts that run their own products (training, experts of
+ * another kind) on the library's routing, and for pm_experts_rows, which wants gathered rows.
+ * Rows are f32, f16 or bf16; sums are f32, in ascending k, the same bits in every run.
+ *
+ * All pointers are DEVICE pointers of the context's GPU. The calls allocate nothing, are queued on
+ * the context's stream, are not waited for, and can be recorded into a CUDA graph. Buffers of one
+ * call must not overlap, except where said. An expert id or a row position in a device buffer that
+ * does not exist is left out and reported by the next pm_sync (PM_ERR_INVALID). */
+#define PM_ROWS_NONE 0xffffffffu /* expert id: a pair without an expert (the padding of a batch);
+                                    position: a pair without a row */
+#define PM_ROWS_MAX_ALIGN 256
+typedef struct pm_rows_desc {
+  int32_t dtype;        /* PM_TYPE_F32, _F16 or _BF16: tokens, rows and their gradients       */
+  int32_t d;            /* values of a row, 1 .. PM_MAX_D                                      */
+  int32_t top_k;        /* pairs of a token, 1 .. PM_MAX_TOPK                                  */
+  int32_t n_exp;        /* expert ids are 0 .. n_exp - 1 (PM_MAX_EXPERTS at most)              */
+  int32_t first_expert; /* pairs of experts [first, first + n_local) have rows,                */
+  int32_t n_local;      /* the others do not (another GPU serves them); 0 = all experts        */
+  int32_t align;        /* every expert's rows start on a multiple of this, 1 .. 256           */
+  int32_t reserved;     /* 0                                                                   */
+  int64_t x_stride;     /* values from a token's row to the next (x, y, add, dx, dy); 0 = d    */
+  int64_t rows_stride;  /* values from a row to the next (rows, drows); 0 = d                  */
+} pm_rows_desc;
+/* The plan of one dispatch, in the caller's device buffers. */
+typedef struct pm_rows_plan {
+  uint32_t *offset;     /* [n_local + 1] first row of each expert; the end of the last         */
+  uint32_t *count;      /* [n_local] rows of each expert that hold a pair; padding follows     */
+  uint32_t *pos;        /* [T * top_k] row of pair t * top_k + k, or PM_ROWS_NONE              */
+  uint32_t *row_pair;   /* [max_rows] pair of a row, PM_ROWS_NONE in the padding; may be NULL  */
+  uint32_t *row_expert; /* [max_rows] expert id of a row (padding: the group's); may be NULL   */
+  float *row_weight;    /* [max_rows] routing weight of a row, 0 in the padding; may be NULL   */
+  int64_t max_rows;     /* rows that the buffers hold, pm_rows_bound at least                  */
+} pm_rows_plan;
+/* rows that a dispatch of T tokens can need: T * top_k and the padding; negative: PM_ERR_* */
+PM_API int64_t pm_rows_bound(const pm_rows_desc *desc, int32_t T);
+/* Sorts the pairs of ids [T][top_k] by expert (ascending; within an expert in the order of the
+ * pairs) into `plan`, and copies x [T][d] to rows [max_rows][d]: rows[pos[p]] = x[t], times w[p]
+ * with PM_ROWS_SCALE. Padding rows of a group are zeros; what lies behind the last group is left as
+ * it was (in row_pair, row_expert and row_weight too). w [T][top_k]: the scale, and what row_weight
+ * receives (NULL: ones). x and rows both NULL: the plan alone. */
+#define PM_ROWS_SCALE 1u
+PM_API int32_t pm_dispatch_rows(pm_ctx *ctx, const pm_rows_desc *desc, int32_t T, const uint32_t *ids,
+                                const float *w, const pm_rows_plan *plan, const void *x, void *rows,
+                                uint32_t flags);
+/* dx[t] = sum_k w[p] drows[pos[p]] (w NULL: rows were not scaled). dw (with x and w, or NULL):
+ * dw[p] = <drows[pos[p]], x[t]>, 0 for a pair without a row. Of the plan: pos, max_rows. */
+PM_API int32_t pm_dispatch_rows_grad(pm_ctx *ctx, const pm_rows_desc *desc, int32_t T, const pm_rows_plan *plan,
+                                     const float *w, const void *x, const void *drows, void *dx, float *dw);
+/* y[t] = add[t] + sum_k w[p] rows[pos[p]] over the token's pairs that have rows. w NULL: ones (rows
+ * already weighted). add [T][d] NULL: zeros; it may be y itself. Of the plan: pos, max_rows. */
+PM_API int32_t pm_collect_rows(pm_ctx *ctx, const pm_rows_desc *desc, int32_t T, const pm_rows_plan *plan,
+                               const float *w, const void *rows, const void *add, void *y);
+/* drows[pos[p]] = w[p] dy[t], zeros in the padding of the groups; what lies behind the last group is
+ * left as it was. dw (with rows, or NULL): dw[p] = <rows[pos[p]], dy[t]>, 0 for a pair without a
+ * row. Of the plan: pos, max_rows, and with align > 1 offset and count. (The gradient of add is dy.) */
+PM_API int32_t pm_collect_rows_grad(pm_ctx *ctx, const pm_rows_desc *desc, int32_t T, const pm_rows_plan *plan,
+                                    const float *w, const void *rows, const void *dy, void *drows, float *dw);
+
+/* ---- norms before and after a block, its gate and the residual stream --------
+ * No counterpart in the reference, whose engines norm, scale and add in shaders of their own around
+ * the FFN. With x the residual stream in front of the block and f the block's output, for each row
+ *   p = f / sqrt(mean(f^2) + eps_post) * (offset_post + w_post)   with PM_NORM_POST, else p = f
+ *   r = alpha x + beta gate p                                      the stream behind the block
+ *   n = r / sqrt(mean(r^2) + eps_pre) * (offset_pre + w_pre)       with PM_NORM_PRE: the next block's input
+ * Streams are f32, f16 or bf16, arithmetic is f32 (n comes from r before it is rounded; squares beyond f32 overflow to
+ * infinity). Pointers, queueing and recording as for the rows above. */
+#define PM_NORM_POST 1
+#define PM_NORM_PRE 2
+enum {
+  PM_NORM_GATE_NONE = 0,    /* gate = 1                         */
+  PM_NORM_GATE_CHANNEL = 1, /* gate [d], shared by all rows      */
+  PM_NORM_GATE_TOKEN = 2    /* gate [T], one factor for each row */
+};
+typedef struct pm_norm_desc {
+  int32_t dtype;  /* PM_TYPE_F32, _F16 or _BF16: x, f, r, n and their gradients  */
+  int32_t wtype;  /* of w_post, w_pre and gate: PM_TYPE_F32, or as dtype         */
+  int32_t d;      /* 1 .. PM_MAX_D                                               */
+  int32_t flags;  /* PM_NORM_POST | PM_NORM_PRE                                  */
+  int32_t gate;   /* PM_NORM_GATE_*                                              */
+  float eps_post, eps_pre;       /* >= 0                                         */
+  float offset_post, offset_pre; /* 0; 1 where a checkpoint stores weight - 1    */
+  float alpha, beta;             /* residual and block scale                     */
+  int32_t reserved;              /* 0                                            */
+  int64_t x_stride, f_stride, r_stride, n_stride; /* values from a row to the next, 0 = d; a gradient
+                                                     has the stride of what it is the gradient of */
+} pm_norm_desc;
+/* x NULL: zeros. f NULL: the stream alone (r = alpha x; neither PM_NORM_POST nor a gate). w_post, w_pre
+ * NULL: ones (no offset). r NULL: only n is wanted. r may be x or f, n may be x or f, with the same stride. */
+PM_API int32_t pm_block_norm(pm_ctx *ctx, const pm_norm_desc *desc, int32_t T, const void *x, const void *f,
+                             const void *w_post, const void *gate, const void *w_pre, void *r, void *n);
+/* The gradient, from r and f (the streams behind the block and out of it), dr (what arrives at r from
+ * later blocks; NULL: zeros) and dn. dx, df, dw_post [d], dgate [d] or [T], dw_pre [d] (the last three
+ * f32): any may be NULL. f is needed for df, dw_post and dgate, r for PM_NORM_PRE. dx may be dr, df may be f or dn,
+ * with the same stride. scratch: device memory of pm_block_norm_scratch bytes, 16-byte aligned, not
+ * shared with work that can run at the same time. */
+PM_API size_t pm_block_norm_scratch(pm_ctx *ctx, const pm_norm_desc *desc, int32_t T);
+PM_API int32_t pm_block_norm_grad(pm_ctx *ctx, const pm_norm_desc *desc, int32_t T, const void *r, const void *f,
+                                  const void *w_post, const void *gate, const void *w_pre, const void *dr,
+                                  const void *dn, void *dx, void *df, float *dw_post, float *dgate, float *dw_pre,
+                                  void *scratch, size_t scratch_bytes);
+
 /* ---- layer stacks (the benchmark's unit: x <- x + moe(rmsnorm(x)) per layer) */
 /* the engines' layer loop around the FFN (src/moe.rs:1279-1440 `after` ops:
  * rmsnorm, FFN, residual add) reduced to its MoE part */

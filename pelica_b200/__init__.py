@@ -46,6 +46,30 @@ class LayerDesc(C.Structure):
     ]
 
 
+class RowsDesc(C.Structure):
+    """pm_rows_desc"""
+
+    _fields_ = [("dtype", C.c_int32), ("d", C.c_int32), ("top_k", C.c_int32), ("n_exp", C.c_int32),
+                ("first_expert", C.c_int32), ("n_local", C.c_int32), ("align", C.c_int32), ("reserved", C.c_int32),
+                ("x_stride", C.c_int64), ("rows_stride", C.c_int64)]
+
+
+class RowsPlan(C.Structure):
+    """pm_rows_plan: device buffers of the caller"""
+
+    _fields_ = [("offset", C.c_void_p), ("count", C.c_void_p), ("pos", C.c_void_p), ("row_pair", C.c_void_p),
+                ("row_expert", C.c_void_p), ("row_weight", C.c_void_p), ("max_rows", C.c_int64)]
+
+
+class NormDesc(C.Structure):
+    """pm_norm_desc"""
+
+    _fields_ = [("dtype", C.c_int32), ("wtype", C.c_int32), ("d", C.c_int32), ("flags", C.c_int32), ("gate", C.c_int32),
+                ("eps_post", C.c_float), ("eps_pre", C.c_float), ("offset_post", C.c_float), ("offset_pre", C.c_float),
+                ("alpha", C.c_float), ("beta", C.c_float), ("reserved", C.c_int32),
+                ("x_stride", C.c_int64), ("f_stride", C.c_int64), ("r_stride", C.c_int64), ("n_stride", C.c_int64)]
+
+
 class PlanOut(C.Structure):
     """pm_plan_out"""
 
@@ -105,6 +129,14 @@ ABI = {
     "pm_dequant": (C.c_int32, [_VP, C.c_int32, _VP, C.c_size_t, _VP]),
     "pm_quant_act": (C.c_int32, [_VP, C.c_int32, _VP, C.c_size_t, _VP, _VP, _VP]),
     "pm_rmsnorm": (C.c_int32, [_VP, _VP, C.c_int32, C.c_int32, C.c_float, _VP]),
+    "pm_rows_bound": (C.c_int64, [C.POINTER(RowsDesc), C.c_int32]),
+    "pm_dispatch_rows": (C.c_int32, [_VP, C.POINTER(RowsDesc), C.c_int32, _VP, _VP, C.POINTER(RowsPlan), _VP, _VP, C.c_uint32]),
+    "pm_dispatch_rows_grad": (C.c_int32, [_VP, C.POINTER(RowsDesc), C.c_int32, C.POINTER(RowsPlan)] + [_VP] * 5),
+    "pm_collect_rows": (C.c_int32, [_VP, C.POINTER(RowsDesc), C.c_int32, C.POINTER(RowsPlan)] + [_VP] * 4),
+    "pm_collect_rows_grad": (C.c_int32, [_VP, C.POINTER(RowsDesc), C.c_int32, C.POINTER(RowsPlan)] + [_VP] * 5),
+    "pm_block_norm": (C.c_int32, [_VP, C.POINTER(NormDesc), C.c_int32] + [_VP] * 7),
+    "pm_block_norm_scratch": (C.c_size_t, [_VP, C.POINTER(NormDesc), C.c_int32]),
+    "pm_block_norm_grad": (C.c_int32, [_VP, C.POINTER(NormDesc), C.c_int32] + [_VP] * 13 + [C.c_size_t]),
     "pm_stack_create": (C.c_int32, [_VP, C.POINTER(_VP), C.c_int32, C.c_float, C.POINTER(_VP)]),
     "pm_stack_destroy": (C.c_int32, [_VP]),
     "pm_stack_forward": (C.c_int32, [_VP, _VP, C.c_int32, _VP]),
@@ -499,6 +531,91 @@ class MoeLayer:
         _check(self.lib.pm_combine(self.h, _ptr(pair_out), _ptr(ids), _ptr(w), _ptr(so), T, _ptr(y),
                                    PM_FWD_ACCUMULATE if acc else 0))
         return y
+
+
+STREAM_TYPES = {"f32": synth.F32, "f16": synth.F16, "bf16": synth.BF16}
+ROWS_NONE = 0xFFFFFFFF
+PM_ROWS_SCALE = 1
+PM_NORM_POST, PM_NORM_PRE = 1, 2
+NORM_GATES = {"none": 0, "channel": 1, "token": 2}
+
+
+def _dev(p):
+    """A device pointer: an address, a DevBuf, or anything with its address in `ptr`; None stays None."""
+    return p if p is None or isinstance(p, int) else p.ptr
+
+
+class Rows:
+    """Tokens sorted by expert and back, with gradients (pm_dispatch_rows, pm_collect_rows). All buffers are device
+    memory of the context's GPU; calls are queued on its stream and allocate nothing."""
+
+    def __init__(self, ctx: Context, d: int, top_k: int, n_exp: int, dtype: str = "f32", first_expert: int = 0, n_local: int = 0,
+                 align: int = 1, x_stride: int = 0, rows_stride: int = 0):
+        self.ctx, self.lib = ctx, ctx.lib
+        self.desc = RowsDesc(STREAM_TYPES[dtype], d, top_k, n_exp, first_expert, n_local, align, 0, x_stride, rows_stride)
+        self.bound(0)
+
+    def bound(self, T: int) -> int:
+        """Rows that T tokens can need, the padding of the groups included."""
+        n = self.lib.pm_rows_bound(C.byref(self.desc), T)
+        if n < 0:
+            _check(n)
+        return n
+
+    def plan(self, max_rows: int, offset, count, pos, row_pair=None, row_expert=None, row_weight=None) -> RowsPlan:
+        """The buffers of a plan: offset [n_local + 1], count [n_local], pos [T, top_k], the others [max_rows]."""
+        return RowsPlan(*(_dev(p) for p in (offset, count, pos, row_pair, row_expert, row_weight)), max_rows)
+
+    def dispatch(self, T: int, ids, plan: RowsPlan, x=None, rows=None, w=None, scale: bool = True):
+        """Fills the plan from ids [T, top_k]; rows[pos] = x[t], times w with `scale` and w given."""
+        flags = PM_ROWS_SCALE if scale and w is not None else 0
+        _check(self.lib.pm_dispatch_rows(self.ctx.h, C.byref(self.desc), T, _dev(ids), _dev(w), C.byref(plan), _dev(x), _dev(rows), flags))
+
+    def dispatch_grad(self, T: int, plan: RowsPlan, drows, dx, w=None, x=None, dw=None):
+        """dx[t] = sum_k w drows[pos]; dw = <drows[pos], x[t]>."""
+        _check(self.lib.pm_dispatch_rows_grad(self.ctx.h, C.byref(self.desc), T, C.byref(plan), _dev(w), _dev(x), _dev(drows), _dev(dx),
+                                              _dev(dw)))
+
+    def collect(self, T: int, plan: RowsPlan, rows, y, w=None, add=None):
+        """y[t] = add[t] + sum_k w rows[pos]."""
+        _check(self.lib.pm_collect_rows(self.ctx.h, C.byref(self.desc), T, C.byref(plan), _dev(w), _dev(rows), _dev(add), _dev(y)))
+
+    def collect_grad(self, T: int, plan: RowsPlan, dy, drows, w=None, rows=None, dw=None):
+        """drows[pos] = w dy[t]; dw = <rows[pos], dy[t]>."""
+        _check(self.lib.pm_collect_rows_grad(self.ctx.h, C.byref(self.desc), T, C.byref(plan), _dev(w), _dev(rows), _dev(dy), _dev(drows),
+                                             _dev(dw)))
+
+
+class BlockNorm:
+    """The norms before and after a block, its gate and the scaled residual stream (pm_block_norm):
+    r = alpha x + beta gate post(f), n = pre(r). Device buffers, as for Rows."""
+
+    def __init__(self, ctx: Context, d: int, dtype: str = "f32", wtype: str = "f32", post: bool = False, pre: bool = True,
+                 gate: str = "none", alpha: float = 1.0, beta: float = 1.0, eps_post: float = 1e-6, eps_pre: float = 1e-6,
+                 offset_post: float = 0.0, offset_pre: float = 0.0, stride: int = 0):
+        self.ctx, self.lib = ctx, ctx.lib
+        self.desc = NormDesc(STREAM_TYPES[dtype], STREAM_TYPES[wtype], d, PM_NORM_POST * bool(post) | PM_NORM_PRE * bool(pre),
+                             NORM_GATES[gate], eps_post, eps_pre, offset_post, offset_pre, alpha, beta, 0, stride, stride, stride, stride)
+        self.scratch_bytes(0)
+
+    def scratch_bytes(self, T: int) -> int:
+        """Bytes of device memory that `grad` of T rows works in."""
+        n = self.lib.pm_block_norm_scratch(self.ctx.h, C.byref(self.desc), T)
+        if n == 0:
+            raise PelicaError(-1, self.lib.pm_last_error().decode())
+        return n
+
+    def forward(self, T: int, x, f, r, n=None, w_post=None, gate=None, w_pre=None):
+        _check(self.lib.pm_block_norm(self.ctx.h, C.byref(self.desc), T, _dev(x), _dev(f), _dev(w_post), _dev(gate), _dev(w_pre), _dev(r),
+                                      _dev(n)))
+
+    def grad(self, T: int, r, f, dr, dn, dx, df, w_post=None, gate=None, w_pre=None, dw_post=None, dgate=None, dw_pre=None, scratch=None,
+             scratch_bytes: int | None = None):
+        if scratch_bytes is None:
+            scratch_bytes = scratch.nbytes if scratch is not None else 0
+        _check(self.lib.pm_block_norm_grad(self.ctx.h, C.byref(self.desc), T, _dev(r), _dev(f), _dev(w_post), _dev(gate), _dev(w_pre),
+                                           _dev(dr), _dev(dn), _dev(dx), _dev(df), _dev(dw_post), _dev(dgate), _dev(dw_pre), _dev(scratch),
+                                           scratch_bytes))
 
 
 class Stack:

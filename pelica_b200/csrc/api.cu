@@ -6,12 +6,15 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <new>
 #include <map>
 #include <memory>
 #include <vector>
 
+#include "block_norm.cuh"
 #include "decode_mega.cuh"
+#include "rows.cuh"
 #include "../../include/pelica_moe_diag.h"
 
 void launch_synth_blocks(const Launch &L, int type, uint8_t *raw, size_t nb, uint64_t seed,
@@ -265,6 +268,9 @@ static int32_t check_dev_err(pm_ctx *c) {
     CU(cudaMemset(c->dev_err, 0, 4));
     if (e == PM_DEVERR_BAD_EXPERT_ID)
       return fail(PM_ERR_INVALID, "an expert id in a device buffer is outside the layer's experts "
+                                  "(its pairs were left out; nothing was read or written out of bounds)");
+    if (e == PM_DEVERR_BAD_ROW)
+      return fail(PM_ERR_INVALID, "a row position in a device buffer is outside the plan's rows "
                                   "(its pairs were left out; nothing was read or written out of bounds)");
     return fail(PM_ERR_TIMEOUT, "a bounded device-side wait gave up (code %d)", e);
   }
@@ -1656,6 +1662,298 @@ extern "C" int32_t pm_rmsnorm(pm_ctx *c, const float *x, int32_t T, int32_t d, f
   launch_rmsnorm(c->launch(), xd, T, d, eps, od);
   CU(cudaGetLastError());
   return out_flush(c, &ob, 1);
+}
+
+// ---------------------------------------------------------------------------
+// rows sorted by expert, block norms: device pointers only, nothing allocated
+// ---------------------------------------------------------------------------
+// a device pointer of the context's GPU, aligned to its values
+static int32_t dev_arg(pm_ctx *c, const char *call, const char *name, const void *p, size_t align) {
+  if (!p) return fail(PM_ERR_INVALID, "%s: %s is null", call, name);
+  cudaPointerAttributes a;
+  if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+    cudaGetLastError();
+    a.type = cudaMemoryTypeUnregistered;
+  }
+  if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged)
+    return fail(PM_ERR_INVALID, "%s: %s must be a device pointer", call, name);
+  if (a.type == cudaMemoryTypeDevice && a.device != c->device)
+    return fail(PM_ERR_INVALID, "%s: %s is memory of device %d, the context is on device %d", call, name, a.device, c->device);
+  if ((uintptr_t)p % align) return fail(PM_ERR_INVALID, "%s: %s is not aligned to %zu bytes", call, name, align);
+  return PM_OK;
+}
+#define DEV_ARG(p, align) TRY(dev_arg(c, call, #p, p, align))
+#define DEV_ARG_OR_NULL(p, align) \
+  do {                            \
+    if (p) DEV_ARG(p, align);     \
+  } while (0)
+
+static size_t stream_type_bytes(int32_t dtype) {
+  return dtype == PM_TYPE_F32 ? 4 : dtype == PM_TYPE_F16 || dtype == PM_TYPE_BF16 ? 2 : 0;
+}
+static bool on_16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+static int32_t rows_desc_check(const char *call, const pm_rows_desc *desc, int32_t T, pm_rows_desc *D) {
+  if (!desc) return fail(PM_ERR_INVALID, "%s: null descriptor", call);
+  *D = *desc;
+  if (!stream_type_bytes(D->dtype)) return fail(PM_ERR_UNSUPPORTED, "%s: type %d (f32, f16 or bf16)", call, D->dtype);
+  if (D->d < 1 || D->d > PM_MAX_D) return fail(PM_ERR_LIMIT, "%s: d=%d outside 1..%d", call, D->d, PM_MAX_D);
+  if (D->top_k < 1 || D->top_k > PM_MAX_TOPK) return fail(PM_ERR_LIMIT, "%s: top_k=%d outside 1..%d", call, D->top_k, PM_MAX_TOPK);
+  if (D->n_exp < 1 || D->n_exp > PM_MAX_EXPERTS) return fail(PM_ERR_LIMIT, "%s: n_exp=%d outside 1..%d", call, D->n_exp, PM_MAX_EXPERTS);
+  if (D->n_local == 0 && D->first_expert == 0) D->n_local = D->n_exp;
+  if (D->first_expert < 0 || D->n_local < 1 || D->first_expert > D->n_exp - D->n_local)
+    return fail(PM_ERR_INVALID, "%s: experts %d..%d of %d", call, D->first_expert, D->first_expert + D->n_local - 1, D->n_exp);
+  if (D->align < 1 || D->align > PM_ROWS_MAX_ALIGN) return fail(PM_ERR_LIMIT, "%s: align=%d outside 1..%d", call, D->align, PM_ROWS_MAX_ALIGN);
+  if (D->reserved) return fail(PM_ERR_INVALID, "%s: reserved field is not 0", call);
+  if (D->x_stride == 0) D->x_stride = D->d;
+  if (D->rows_stride == 0) D->rows_stride = D->d;
+  if (D->x_stride < D->d || D->rows_stride < D->d) return fail(PM_ERR_INVALID, "%s: a stride is below d=%d", call, D->d);
+  return check_T(T);
+}
+static int64_t rows_bound(const pm_rows_desc &D, int32_t T) {
+  const int64_t P = (int64_t)T * D.top_k;
+  return P + (P < D.n_local ? P : D.n_local) * (D.align - 1);
+}
+extern "C" int64_t pm_rows_bound(const pm_rows_desc *desc, int32_t T) {
+  pm_rows_desc D;
+  TRY(rows_desc_check("pm_rows_bound", desc, T, &D));
+  return rows_bound(D, T);
+}
+
+// what every call on a plan checks; *rc.vec: whether the named buffers allow 16-byte accesses
+static int32_t rows_call(pm_ctx *c, const char *call, const pm_rows_desc *desc, int32_t T, const pm_rows_plan *plan, RowsCall *rc) {
+  TRY(rows_desc_check(call, desc, T, &rc->D));
+  if (!c || !plan) return fail(PM_ERR_INVALID, "%s: null context or plan", call);
+  rc->pl = *plan;
+  rc->T = T;
+  rc->err = c->dev_err;
+  const int64_t need = rows_bound(rc->D, T);
+  if (plan->max_rows < need)
+    return fail(PM_ERR_INVALID, "%s: max_rows=%lld, but %d tokens can need %lld rows", call, (long long)plan->max_rows, T, (long long)need);
+  if (plan->max_rows > INT32_MAX) return fail(PM_ERR_LIMIT, "%s: max_rows=%lld", call, (long long)plan->max_rows);
+  CU(cudaSetDevice(c->device));
+  if (T > 0) {
+    const uint32_t *pos = plan->pos;
+    DEV_ARG(pos, 4);
+  }
+  return PM_OK;
+}
+static bool rows_vec(const RowsCall &rc, std::initializer_list<const void *> buffers) {
+  const int64_t v = 16 / (int64_t)stream_type_bytes(rc.D.dtype);
+  bool ok = rc.D.d % v == 0 && rc.D.x_stride % v == 0 && rc.D.rows_stride % v == 0;
+  for (const void *p : buffers) ok = ok && on_16(p);
+  return ok;
+}
+
+extern "C" int32_t pm_dispatch_rows(pm_ctx *c, const pm_rows_desc *desc, int32_t T, const uint32_t *ids, const float *w,
+                                    const pm_rows_plan *plan, const void *x, void *rows, uint32_t flags) {
+  static const char *call = "pm_dispatch_rows";
+  RowsCall rc;
+  TRY(rows_call(c, call, desc, T, plan, &rc));
+  if (flags & ~PM_ROWS_SCALE) return fail(PM_ERR_INVALID, "%s: flags %#x", call, flags);
+  const size_t e = stream_type_bytes(rc.D.dtype);
+  uint32_t *offset = plan->offset, *count = plan->count, *row_pair = plan->row_pair, *row_expert = plan->row_expert;
+  float *row_weight = plan->row_weight;
+  DEV_ARG(offset, 4);
+  DEV_ARG(count, 4);
+  if (T > 0) {
+    DEV_ARG(ids, 4);
+    DEV_ARG_OR_NULL(row_pair, 4);
+    DEV_ARG_OR_NULL(row_expert, 4);
+    DEV_ARG_OR_NULL(row_weight, 4);
+    DEV_ARG_OR_NULL(w, 4);
+    if ((flags & PM_ROWS_SCALE) && !w) return fail(PM_ERR_INVALID, "%s: PM_ROWS_SCALE without w", call);
+    if (x || rows) {
+      DEV_ARG(x, e);
+      DEV_ARG(rows, e);
+    }
+  }
+  rc.vec = rows_vec(rc, {x, rows});
+  CU(launch_rows_dispatch(c->launch(), rc, ids, w, flags & PM_ROWS_SCALE, x, rows));
+  return PM_OK;
+}
+
+extern "C" int32_t pm_dispatch_rows_grad(pm_ctx *c, const pm_rows_desc *desc, int32_t T, const pm_rows_plan *plan, const float *w,
+                                         const void *x, const void *drows, void *dx, float *dw) {
+  static const char *call = "pm_dispatch_rows_grad";
+  RowsCall rc;
+  TRY(rows_call(c, call, desc, T, plan, &rc));
+  if (T == 0) return PM_OK;
+  const size_t e = stream_type_bytes(rc.D.dtype);
+  DEV_ARG(drows, e);
+  DEV_ARG(dx, e);
+  DEV_ARG_OR_NULL(w, 4);
+  DEV_ARG_OR_NULL(dw, 4);
+  if (dw) {
+    DEV_ARG(x, e);
+    DEV_ARG(w, 4);
+  }
+  rc.vec = rows_vec(rc, {dw ? x : nullptr, drows, dx});
+  CU(launch_rows_gather(c->launch(), rc, w, drows, nullptr, x, dx, dw));
+  return PM_OK;
+}
+
+extern "C" int32_t pm_collect_rows(pm_ctx *c, const pm_rows_desc *desc, int32_t T, const pm_rows_plan *plan, const float *w, const void *rows,
+                                   const void *add, void *y) {
+  static const char *call = "pm_collect_rows";
+  RowsCall rc;
+  TRY(rows_call(c, call, desc, T, plan, &rc));
+  if (T == 0) return PM_OK;
+  const size_t e = stream_type_bytes(rc.D.dtype);
+  DEV_ARG(rows, e);
+  DEV_ARG(y, e);
+  DEV_ARG_OR_NULL(w, 4);
+  DEV_ARG_OR_NULL(add, e);
+  rc.vec = rows_vec(rc, {rows, add, y});
+  CU(launch_rows_gather(c->launch(), rc, w, rows, add, nullptr, y, nullptr));
+  return PM_OK;
+}
+
+extern "C" int32_t pm_collect_rows_grad(pm_ctx *c, const pm_rows_desc *desc, int32_t T, const pm_rows_plan *plan, const float *w,
+                                        const void *rows, const void *dy, void *drows, float *dw) {
+  static const char *call = "pm_collect_rows_grad";
+  RowsCall rc;
+  TRY(rows_call(c, call, desc, T, plan, &rc));
+  if (T == 0) return PM_OK;
+  const size_t e = stream_type_bytes(rc.D.dtype);
+  DEV_ARG(dy, e);
+  DEV_ARG(drows, e);
+  DEV_ARG_OR_NULL(w, 4);
+  DEV_ARG_OR_NULL(dw, 4);
+  if (dw) DEV_ARG(rows, e);
+  if (rc.D.align > 1) {
+    const uint32_t *offset = plan->offset, *count = plan->count;
+    DEV_ARG(offset, 4);
+    DEV_ARG(count, 4);
+  }
+  rc.vec = rows_vec(rc, {dw ? rows : nullptr, dy, drows});
+  CU(launch_rows_spread(c->launch(), rc, w, dy, rows, drows, dw));
+  return PM_OK;
+}
+
+static int32_t norm_desc_check(const char *call, const pm_norm_desc *desc, int32_t T, pm_norm_desc *D) {
+  if (!desc) return fail(PM_ERR_INVALID, "%s: null descriptor", call);
+  *D = *desc;
+  if (!stream_type_bytes(D->dtype)) return fail(PM_ERR_UNSUPPORTED, "%s: type %d (f32, f16 or bf16)", call, D->dtype);
+  if (D->wtype != PM_TYPE_F32 && D->wtype != D->dtype) return fail(PM_ERR_UNSUPPORTED, "%s: weight type %d (f32, or as the streams)", call, D->wtype);
+  if (D->d < 1 || D->d > PM_MAX_D) return fail(PM_ERR_LIMIT, "%s: d=%d outside 1..%d", call, D->d, PM_MAX_D);
+  if (D->flags & ~(PM_NORM_POST | PM_NORM_PRE)) return fail(PM_ERR_INVALID, "%s: flags %#x", call, D->flags);
+  if (D->gate < PM_NORM_GATE_NONE || D->gate > PM_NORM_GATE_TOKEN) return fail(PM_ERR_INVALID, "%s: gate %d", call, D->gate);
+  if (!(D->eps_post >= 0.0f) || !(D->eps_pre >= 0.0f)) return fail(PM_ERR_INVALID, "%s: eps below 0 or not a number", call);
+  if (D->reserved) return fail(PM_ERR_INVALID, "%s: reserved field is not 0", call);
+  for (int64_t *s : {&D->x_stride, &D->f_stride, &D->r_stride, &D->n_stride}) {
+    if (*s == 0) *s = D->d;
+    if (*s < D->d) return fail(PM_ERR_INVALID, "%s: a stride is below d=%d", call, D->d);
+  }
+  return check_T(T);
+}
+static bool norm_vec(const pm_norm_desc &D, std::initializer_list<const void *> buffers) {
+  const int64_t v = 16 / (int64_t)stream_type_bytes(D.dtype);
+  bool ok = D.d % v == 0 && D.x_stride % v == 0 && D.f_stride % v == 0 && D.r_stride % v == 0 && D.n_stride % v == 0;
+  for (const void *p : buffers) ok = ok && on_16(p);
+  return ok;
+}
+// what both directions check of the weights
+static int32_t norm_weights_check(pm_ctx *c, const char *call, const pm_norm_desc &D, const void *f, const void *w_post, const void *gate,
+                                  const void *w_pre) {
+  const size_t e = stream_type_bytes(D.wtype);
+  if (!f && ((D.flags & PM_NORM_POST) || D.gate != PM_NORM_GATE_NONE)) return fail(PM_ERR_INVALID, "%s: a post norm or gate without f", call);
+  if (D.flags & PM_NORM_POST) DEV_ARG_OR_NULL(w_post, e);
+  if (D.flags & PM_NORM_PRE) DEV_ARG_OR_NULL(w_pre, e);
+  if (D.gate != PM_NORM_GATE_NONE) DEV_ARG(gate, e);
+  return PM_OK;
+}
+
+extern "C" int32_t pm_block_norm(pm_ctx *c, const pm_norm_desc *desc, int32_t T, const void *x, const void *f, const void *w_post, const void *gate,
+                                 const void *w_pre, void *r, void *n) {
+  static const char *call = "pm_block_norm";
+  NormCall nc = {};
+  TRY(norm_desc_check(call, desc, T, &nc.D));
+  if (!c) return fail(PM_ERR_INVALID, "%s: null context", call);
+  if (T == 0) return PM_OK;
+  CU(cudaSetDevice(c->device));
+  const size_t e = stream_type_bytes(nc.D.dtype);
+  if (!x && !f) return fail(PM_ERR_INVALID, "%s: neither x nor f", call);
+  DEV_ARG_OR_NULL(x, e);
+  DEV_ARG_OR_NULL(f, e);
+  TRY(norm_weights_check(c, call, nc.D, f, w_post, gate, w_pre));
+  if (nc.D.flags & PM_NORM_PRE) {
+    DEV_ARG(n, e);
+    DEV_ARG_OR_NULL(r, e);
+  } else {
+    DEV_ARG(r, e);
+    n = nullptr;
+  }
+  nc.T = T;
+  nc.x = x;
+  nc.f = f;
+  nc.w_post = nc.D.flags & PM_NORM_POST ? w_post : nullptr;
+  nc.gate = nc.D.gate != PM_NORM_GATE_NONE ? gate : nullptr;
+  nc.w_pre = nc.D.flags & PM_NORM_PRE ? w_pre : nullptr;
+  nc.r = r;
+  nc.n = n;
+  nc.vec = norm_vec(nc.D, {x, f, nc.w_post, nc.D.gate == PM_NORM_GATE_CHANNEL ? gate : nullptr, nc.w_pre, r, n});
+  CU(launch_block_norm(c->launch(), nc));
+  return PM_OK;
+}
+
+extern "C" size_t pm_block_norm_scratch(pm_ctx *c, const pm_norm_desc *desc, int32_t T) {
+  pm_norm_desc D;
+  if (!c || norm_desc_check("pm_block_norm_scratch", desc, T, &D) != PM_OK) return 0;
+  const size_t b = norm_parts_floats(D, T, c->n_sm) * sizeof(float);
+  return b > 16 ? b : 16;
+}
+
+extern "C" int32_t pm_block_norm_grad(pm_ctx *c, const pm_norm_desc *desc, int32_t T, const void *r, const void *f, const void *w_post,
+                                      const void *gate, const void *w_pre, const void *dr, const void *dn, void *dx, void *df, float *dw_post,
+                                      float *dgate, float *dw_pre, void *scratch, size_t scratch_bytes) {
+  static const char *call = "pm_block_norm_grad";
+  NormCall nc = {};
+  TRY(norm_desc_check(call, desc, T, &nc.D));
+  if (!c) return fail(PM_ERR_INVALID, "%s: null context", call);
+  CU(cudaSetDevice(c->device));
+  const size_t e = stream_type_bytes(nc.D.dtype);
+  const bool post = nc.D.flags & PM_NORM_POST, pre = nc.D.flags & PM_NORM_PRE;
+  if (dw_post && !post) return fail(PM_ERR_INVALID, "%s: dw_post without PM_NORM_POST", call);
+  if (dw_pre && !pre) return fail(PM_ERR_INVALID, "%s: dw_pre without PM_NORM_PRE", call);
+  if (dgate && nc.D.gate == PM_NORM_GATE_NONE) return fail(PM_ERR_INVALID, "%s: dgate without a gate", call);
+  if (T > 0) {
+    if (!f && df) return fail(PM_ERR_INVALID, "%s: df without f", call);
+    if (pre) {
+      DEV_ARG(r, e);
+      DEV_ARG(dn, e);
+    }
+    DEV_ARG_OR_NULL(f, e);
+    DEV_ARG_OR_NULL(dr, e);
+    TRY(norm_weights_check(c, call, nc.D, f, w_post, gate, w_pre));
+    DEV_ARG_OR_NULL(dx, e);
+    DEV_ARG_OR_NULL(df, e);
+  }
+  DEV_ARG_OR_NULL(dw_post, 4);
+  DEV_ARG_OR_NULL(dw_pre, 4);
+  DEV_ARG_OR_NULL(dgate, 4);
+  const size_t need = norm_parts_floats(nc.D, T, c->n_sm) * sizeof(float);
+  if (dw_post || dw_pre || (dgate && nc.D.gate == PM_NORM_GATE_CHANNEL)) {
+    if (scratch_bytes < need) return fail(PM_ERR_INVALID, "%s: scratch of %zu bytes, %zu needed", call, scratch_bytes, need);
+    if (need) DEV_ARG(scratch, 16);
+  }
+  nc.T = T;
+  nc.x = pre ? r : nullptr;
+  nc.f = f;
+  nc.w_post = post ? w_post : nullptr;
+  nc.gate = nc.D.gate != PM_NORM_GATE_NONE ? gate : nullptr;
+  nc.w_pre = pre ? w_pre : nullptr;
+  nc.dr = dr;
+  nc.dn = pre ? dn : nullptr;
+  nc.dx = dx;
+  nc.df = df;
+  nc.dw_post = dw_post;
+  nc.dgate = dgate;
+  nc.dw_pre = dw_pre;
+  nc.parts = (float *)scratch;
+  nc.vec = norm_vec(nc.D, {nc.x, f, nc.w_post, nc.D.gate == PM_NORM_GATE_CHANNEL ? gate : nullptr, nc.w_pre, dr, nc.dn, dx, df});
+  CU(launch_block_norm_grad(c->launch(), nc));
+  return PM_OK;
 }
 
 // ---------------------------------------------------------------------------
