@@ -1844,6 +1844,7 @@ static int32_t norm_desc_check(const char *call, const pm_norm_desc *desc, int32
   for (int64_t *s : {&D->x_stride, &D->f_stride, &D->r_stride, &D->n_stride}) {
     if (*s == 0) *s = D->d;
     if (*s < D->d) return fail(PM_ERR_INVALID, "%s: a stride is below d=%d", call, D->d);
+    if (*s > INT32_MAX) return fail(PM_ERR_LIMIT, "%s: a stride is beyond 31 bits", call);
   }
   return check_T(T);
 }
@@ -1885,6 +1886,7 @@ extern "C" int32_t pm_block_norm(pm_ctx *c, const pm_norm_desc *desc, int32_t T,
     n = nullptr;
   }
   nc.T = T;
+  nc.inv_d = 1.0f / (float)nc.D.d;
   nc.x = x;
   nc.f = f;
   nc.w_post = nc.D.flags & PM_NORM_POST ? w_post : nullptr;
@@ -1938,6 +1940,7 @@ extern "C" int32_t pm_block_norm_grad(pm_ctx *c, const pm_norm_desc *desc, int32
     if (need) DEV_ARG(scratch, 16);
   }
   nc.T = T;
+  nc.inv_d = 1.0f / (float)nc.D.d;
   nc.x = pre ? r : nullptr;
   nc.f = f;
   nc.w_post = post ? w_post : nullptr;

@@ -17,18 +17,29 @@
 namespace cg = cooperative_groups;
 
 // A thread holds 8 values of a row; a row's group has tpr threads (whole warps) in each of cl CTAs (a cluster, for rows of
-// more than 8,192 values), a CTA has rpb groups, each with rows of its own.
+// more than 8,192 values), a CTA has rpb groups, each with rows of its own. Rows of a group follow one another; a thread
+// copies its own values of the next ones into its own slots of shared memory (cp.async) while it works on one, so that the bytes
+// in flight do not depend on registers and no thread waits for another's copy.
 #define NORM_VALUES 8
+#define NORM_GRAD_THREADS 896  // ... backward: 72
+#define NORM_THREADS 1024      // threads resident on an SM, forward: 64 registers each
+#define NORM_SMEM 233472      // bytes of shared memory of an SM, of which every CTA takes
+#define NORM_SMEM_CTA 2560    // ... these for its sums and for itself
 struct NormShape {
-  int tpr, rpb, cl;
+  int tpr, rpb, cl;   // threads of a row's group in a CTA, groups of a CTA, CTAs of a row
+  int stages;         // rows in a group's ring, 0: none
+  int slots;          // of shared memory, a thread
+  int per_sm;         // CTAs resident on an SM
+  int threads() const { return tpr * rpb; }
 };
-static NormShape norm_shape(int d) {
-  NormShape s;
+static NormShape norm_shape(int d, int sm_threads) {
+  NormShape s = {};
   const int need = (d + NORM_VALUES - 1) / NORM_VALUES;
   s.cl = 1;
-  while ((need + s.cl - 1) / s.cl > 1024) s.cl *= 2;
+  while ((need + s.cl - 1) / s.cl > sm_threads) s.cl *= 2;
   s.tpr = ((need + s.cl - 1) / s.cl + 31) / 32 * 32;
   s.rpb = s.cl == 1 && s.tpr < 256 ? 256 / s.tpr : 1;
+  s.per_sm = sm_threads / s.threads();
   return s;
 }
 
@@ -37,43 +48,63 @@ struct NormPlace {
   int lane, warp, group, tpr, cl, rank, col0;
 };
 
-// Sums of N values over a row's group, in every thread: lanes, then warps through red (two turns used alternately,
-// so that one barrier a sum is enough), then the cluster's CTAs.
-template <int N, bool CLUSTER>
-__device__ __forceinline__ void norm_sum(float (&v)[N], const NormPlace &at, float (*red)[32][N], float (*peer)[8][N], int &turn) {
+// sums over a warp: of one value, in every lane; of three, value q in the lanes with lane & 3 == q
+template <int N> __device__ __forceinline__ float norm_warp_sums(const float (&v)[N], int lane) {
+  static_assert(N == 1 || N == 3, "");
+  if constexpr (N == 1) return pm_warp_sum_16_1(v[0]);
+  else {  // lanes of a quad keep one value each: 2 + 1 + 3 exchanges for 15
+    const bool b0 = lane & 1, b1 = lane & 2;
+    const float a = __fadd_rn(b0 ? v[1] : v[0], __shfl_xor_sync(PM_FULL, b0 ? v[0] : v[1], 1));  // values 0, 1
+    const float c = __fadd_rn(b0 ? 0.0f : v[2], __shfl_xor_sync(PM_FULL, b0 ? v[2] : 0.0f, 1));  // value 2
+    float s = __fadd_rn(b1 ? c : a, __shfl_xor_sync(PM_FULL, b1 ? a : c, 2));
 #pragma unroll
-  for (int i = 0; i < N; i++) v[i] = pm_warp_sum_16_1(v[i]);
-  const int warps = at.tpr >> 5;
-  if (warps == 1 && !CLUSTER) return;
-  float (*mine)[N] = red[turn] + at.group * warps;
-  if (at.lane == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i++) mine[at.warp][i] = v[i];
+    for (int o = 4; o < 32; o <<= 1) s = __fadd_rn(s, __shfl_xor_sync(PM_FULL, s, o));
+    return s;
   }
-  if constexpr (CLUSTER) __syncthreads();
-  else asm volatile("bar.sync %0, %1;" ::"r"(at.group + 1), "r"(at.tpr) : "memory");
+}
+
+// Sums of N values over a row's group, in every thread: lanes, then warps through red (two turns used alternately, so that one
+// barrier a sum is enough), then the cluster's CTAs.
+template <int N> using NormRed = float[2][N == 1 ? 1 : 4][32];
+template <int N> using NormPeer = float[2][8][N];
+template <int N, bool CLUSTER>
+__device__ __forceinline__ void norm_sum(float (&v)[N], const NormPlace &at, NormRed<N> &red, NormPeer<N> &peer, int &turn) {
+  constexpr int Q = N == 1 ? 1 : 4;
+  float s = norm_warp_sums<N>(v, at.lane);
+  const int warps = at.tpr >> 5;
+  if (warps > 1 || CLUSTER) {
+    const int first = at.group * warps;
+    if (at.lane < Q) red[turn][at.lane][first + at.warp] = s;
+    if constexpr (CLUSTER) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(at.group + 1), "r"(at.tpr) : "memory");
 #pragma unroll
-  for (int i = 0; i < N; i++) v[i] = pm_warp_sum_16_1(at.lane < warps ? mine[at.lane][i] : 0.0f);
+    for (int i = 0; i < N; i++) v[i] = at.lane < warps ? red[turn][i][first + at.lane] : 0.0f;
+    s = norm_warp_sums<N>(v, at.lane);
+  }
   if constexpr (CLUSTER) {
     cg::cluster_group cluster = cg::this_cluster();
-    if (at.warp == 0 && at.lane < at.cl) {
-      float *to = cluster.map_shared_rank(&peer[turn][at.rank][0], at.lane);
-#pragma unroll
-      for (int i = 0; i < N; i++) to[i] = v[i];
-    }
+    // lane i * Q + q of the first warp gives sum q to CTA i
+    if (at.warp == 0 && at.lane < at.cl * Q && (at.lane & (Q - 1)) < N)
+      cluster.map_shared_rank(&peer[turn][at.rank][0], at.lane / Q)[at.lane & (Q - 1)] = s;
     cluster.sync();
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      float s = 0.0f;
-      for (int q = 0; q < at.cl; q++) s = __fadd_rn(s, peer[turn][q][i]);
-      v[i] = s;
+      float sum = 0.0f;
+      for (int q = 0; q < at.cl; q++) sum = __fadd_rn(sum, peer[turn][q][i]);
+      v[i] = sum;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = N == 1 ? s : __shfl_sync(PM_FULL, s, i);
   }
   turn ^= 1;
 }
 
-__device__ __forceinline__ float norm_inv(float sum, int d, float eps) {
-  return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)d), eps)));
+// 1 / sqrt(sum / d + eps): the hardware's estimate and one step of Newton's iteration (left out where it has no value: 0, infinity)
+__device__ __forceinline__ float norm_inv(float sum, float inv_d, float eps) {
+  const float x = __fmaf_rn(sum, inv_d, eps), y = rsqrtf(x);
+  const float e = __fmaf_rn(-__fmul_rn(x, y), y, 1.0f);
+  return fabsf(e) < 1.0f ? __fmaf_rn(__fmul_rn(0.5f, y), e, y) : y;
 }
 
 // the thread's 8 values of a row as vectors of V: vector j is columns col0 + j * step ...
@@ -91,40 +122,103 @@ template <typename E, int V> struct NormRow {
       }
     }
   }
-  __device__ __forceinline__ void widen(float (&f)[NORM_VALUES]) const {
+  __device__ __forceinline__ F8 widen() const {
+    F8 f;
 #pragma unroll
-    for (int j = 0; j < J; j++) {
-      float g[V];
-      pm_widen<E, V>(v[j], g);
-#pragma unroll
-      for (int i = 0; i < V; i++) f[j * V + i] = g[i];
+    for (int i = 0; i < 4; i++) {
+      if constexpr (V == 1) f.p[i] = pm_pack2(pm_to_f32(v[2 * i].v[0]), pm_to_f32(v[2 * i + 1].v[0]));
+      else f.p[i] = pm_widen2(&v[2 * i / V].v[2 * i % V]);
     }
+    return f;
   }
-  __device__ __forceinline__ static void store(void *base, size_t at, const NormPlace &p, int d, const float (&f)[NORM_VALUES]) {
+  __device__ __forceinline__ static void store(void *base, size_t at, const NormPlace &p, int d, const F8 &f) {
+    float g[NORM_VALUES];
+#pragma unroll
+    for (int i = 0; i < 4; i++) pm_unpack2(f.p[i], g[2 * i], g[2 * i + 1]);
 #pragma unroll
     for (int j = 0; j < J; j++) {
       const int col = p.col0 + j * p.tpr * p.cl * V;
-      float g[V];
+      float h[V];
 #pragma unroll
-      for (int i = 0; i < V; i++) g[i] = f[j * V + i];
-      if (col < d) pm_store<E, V>((E *)base + at + col, pm_narrow<E, V>(g));
+      for (int i = 0; i < V; i++) h[i] = g[j * V + i];
+      if (col < d) pm_store<E, V>((E *)base + at + col, pm_narrow<E, V>(h));
     }
   }
 };
-// weights of the thread's columns, offset added; `one` where there are none
+// weights of the thread's columns, offset added; ones where there are none
 template <typename W, int V>
-__device__ __forceinline__ void norm_weights(float (&f)[NORM_VALUES], const void *w, float offset, const NormPlace &p, int d) {
-  if (!w) {
-#pragma unroll
-    for (int i = 0; i < NORM_VALUES; i++) f[i] = 1.0f;
-    return;
-  }
+__device__ __forceinline__ F8 norm_weights(const void *w, float offset, const NormPlace &p, int d) {
+  if (!w) return F8::all(1.0f);
   NormRow<W, V> r;
   r.load(w, 0, p, d);
-  r.widen(f);
-#pragma unroll
-  for (int i = 0; i < NORM_VALUES; i++) f[i] = __fadd_rn(f[i], offset);
+  return r.widen() + F8::all(offset);
 }
+
+// The thread's slots of shared memory: 16 bytes each, `pitch` bytes (all threads' of the CTA) apart. Addresses of the shared
+// window throughout; the accesses are volatile: a value that is read a second time is read, not kept in registers.
+struct NormSlots {
+  uint32_t mine, pitch;
+  __device__ __forceinline__ uint32_t at(int i) const { return mine + i * pitch; }
+  __device__ __forceinline__ static uint4 get(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+  }
+  __device__ __forceinline__ static void put(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+  }
+  __device__ __forceinline__ void put8(int i, const F8 &f) const {
+    asm volatile("st.shared.v2.u64 [%0], {%1, %2};" ::"r"(at(i)), "l"(f.p[0]), "l"(f.p[1]) : "memory");
+    asm volatile("st.shared.v2.u64 [%0], {%1, %2};" ::"r"(at(i + 1)), "l"(f.p[2]), "l"(f.p[3]) : "memory");
+  }
+  __device__ __forceinline__ F8 get8(int i) const {
+    F8 f;
+    asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(f.p[0]), "=l"(f.p[1]) : "r"(at(i)));
+    asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(f.p[2]), "=l"(f.p[3]) : "r"(at(i + 1)));
+    return f;
+  }
+};
+__device__ __forceinline__ NormSlots norm_slots(uint4 *all) { return {(uint32_t)__cvta_generic_to_shared(all + threadIdx.x), blockDim.x * 16}; }
+// The streams of a group's rows: with RING, stream k of a stage is slot k * J behind the stage's `row`; without, a load.
+template <typename E, int V, bool RING> struct NormRing {
+  static constexpr int J = NORM_VALUES / V;
+  NormSlots slots;
+  int first, streams, stages;
+  // (columns behind the row are never copied: they stay zero)
+  __device__ __forceinline__ void clear() const {
+    if constexpr (RING)
+      for (int i = 0; i < stages * streams * J; i++) NormSlots::put(slots.at(first + i), make_uint4(0, 0, 0, 0));
+  }
+  __device__ __forceinline__ uint32_t row(int stage) const { return slots.at(first + stage * streams * J); }
+  __device__ __forceinline__ void copy(uint32_t row, int k, const void *base, size_t at, const NormPlace &p, int d) const {
+    if constexpr (RING) {
+#pragma unroll
+      for (int j = 0; j < J; j++) {
+        const int col = p.col0 + j * p.tpr * p.cl * V;
+        if (col < d) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(row + (k * J + j) * slots.pitch), "l"((const E *)base + at + col) : "memory");
+      }
+    }
+  }
+  __device__ __forceinline__ static void commit() {
+    if constexpr (RING) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // until the oldest of the rows in flight is here
+  __device__ __forceinline__ void wait() const {
+    if constexpr (RING) {
+      if (stages >= 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+  }
+  __device__ __forceinline__ void get(NormRow<E, V> &r, uint32_t row, int k, const void *base, size_t at, const NormPlace &p, int d) const {
+    if constexpr (RING) {
+#pragma unroll
+      for (int j = 0; j < J; j++) *(uint4 *)&r.v[j] = NormSlots::get(row + (k * J + j) * slots.pitch);
+    } else {
+      r.load(base, at, p, d);
+    }
+  }
+};
 
 template <bool CLUSTER> __device__ __forceinline__ NormPlace norm_place(int tpr, int cl, int v) {
   NormPlace p;
@@ -139,177 +233,206 @@ template <bool CLUSTER> __device__ __forceinline__ NormPlace norm_place(int tpr,
   return p;
 }
 
+// (strides are 31 bits: one multiplication)
+__device__ __forceinline__ size_t norm_row(int t, int64_t stride) { return (size_t)(uint32_t)t * (uint32_t)stride; }
+
 template <typename W> __device__ __forceinline__ float norm_token_gate(const NormCall &c, int t) {
   return c.D.gate == PM_NORM_GATE_TOKEN ? pm_to_f32(((const W *)c.gate)[t]) : 1.0f;
 }
 
-template <typename E, typename W, int V, bool CLUSTER>
-__global__ void __launch_bounds__(1024) k_block_norm(NormCall c, int tpr, int rpb, int cl) {
+// What a call has, known when the kernel is compiled: a row costs half the instructions where the streams need no questions.
+//   NORM_ANY       whatever the call gives
+//   NORM_SANDWICH  both norms and every stream
+//   NORM_BEFORE    the norm before the next block only, every stream
+enum NormMode { NORM_ANY, NORM_SANDWICH, NORM_BEFORE };
+
+template <typename E, typename W, int V, bool CLUSTER, bool RING, NormMode MODE>
+__global__ void __launch_bounds__(NORM_THREADS) k_block_norm(NormCall c, int tpr, int rpb, int cl, int stages) {
   pm_pdl();
-  __shared__ float red[2][32][1], peer[2][8][1];
+  extern __shared__ uint4 slots[];
+  __shared__ NormRed<1> red;
+  __shared__ NormPeer<1> peer;
   const NormPlace at = norm_place<CLUSTER>(tpr, cl, V);
   const int d = c.D.d, groups = (int)(gridDim.x / at.cl) * rpb;
-  const bool post = c.D.flags & PM_NORM_POST, pre = c.D.flags & PM_NORM_PRE;
-  float wp[NORM_VALUES], wn[NORM_VALUES];  // gate and post weight; pre weight
-  norm_weights<W, V>(wp, post ? c.w_post : nullptr, c.D.offset_post, at, d);
-  norm_weights<W, V>(wn, pre ? c.w_pre : nullptr, c.D.offset_pre, at, d);
-  if (c.D.gate == PM_NORM_GATE_CHANNEL) {
-    float g[NORM_VALUES];
-    norm_weights<W, V>(g, c.gate, 0.0f, at, d);
-#pragma unroll
-    for (int i = 0; i < NORM_VALUES; i++) wp[i] = __fmul_rn(wp[i], g[i]);
-  }
-  int turn = 0;
-  for (int t = (int)(blockIdx.x / at.cl) * rpb + at.group; t < c.T; t += groups) {
-    NormRow<E, V> xr, fr;
-    float r[NORM_VALUES], p[NORM_VALUES], sum[1];
-    if (c.f) fr.load(c.f, (size_t)t * c.D.f_stride, at, d);
-    if (c.x) xr.load(c.x, (size_t)t * c.D.x_stride, at, d);
-    if (c.x) {
-      xr.widen(r);
-#pragma unroll
-      for (int i = 0; i < NORM_VALUES; i++) r[i] = __fmul_rn(c.D.alpha, r[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < NORM_VALUES; i++) r[i] = 0.0f;
+  constexpr bool ANY = MODE == NORM_ANY;
+  const bool post = ANY ? c.D.flags & PM_NORM_POST : MODE == NORM_SANDWICH, pre = ANY ? c.D.flags & PM_NORM_PRE : true;
+  const bool has_x = ANY ? c.x != nullptr : true, has_f = ANY ? c.f != nullptr : true, has_r = ANY ? c.r != nullptr : true;
+  const int i_x = has_f ? 1 : 0;
+  const NormRing<E, V, RING> ring = {norm_slots(slots), 0, i_x + (has_x ? 1 : 0), stages};
+  const int t0 = (int)(blockIdx.x / at.cl) * rpb + at.group;
+  auto copy = [&](int stage, int t) {
+    if (t < c.T) {
+      uint32_t row = ring.row(stage);
+      if (has_f) ring.copy(row, 0, c.f, norm_row(t, c.D.f_stride), at, d);
+      if (has_x) ring.copy(row, i_x, c.x, norm_row(t, c.D.x_stride), at, d);
     }
-    if (c.f) {
-      fr.widen(p);
+    ring.commit();
+  };
+  ring.clear();
+  if constexpr (RING)
+    for (int s = 0; s < stages; s++) copy(s, t0 + s * groups);
+  F8 wp = norm_weights<W, V>(post ? c.w_post : nullptr, c.D.offset_post, at, d);  // gate and post weight
+  const F8 wn = norm_weights<W, V>(pre ? c.w_pre : nullptr, c.D.offset_pre, at, d);
+  if (c.D.gate == PM_NORM_GATE_CHANNEL) wp = wp * norm_weights<W, V>(c.gate, 0.0f, at, d);
+  int turn = 0, stage = 0;
+  for (int t = t0; t < c.T; t += groups) {
+    NormRow<E, V> xr, fr;
+    ring.wait();
+    const uint32_t row = ring.row(stage);
+    if (has_f) ring.get(fr, row, 0, c.f, norm_row(t, c.D.f_stride), at, d);
+    if (has_x) ring.get(xr, row, i_x, c.x, norm_row(t, c.D.x_stride), at, d);
+    if constexpr (RING) {
+      copy(stage, t + stages * groups);
+      stage = stage + 1 == stages ? 0 : stage + 1;
+    }
+    F8 r = has_x ? xr.widen() * c.D.alpha : F8::all(0.0f);
+    if (has_f) {
+      const F8 f = fr.widen();
       float s = __fmul_rn(c.D.beta, norm_token_gate<W>(c, t));
       if (post) {
-        sum[0] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NORM_VALUES; i++) sum[0] = __fmaf_rn(p[i], p[i], sum[0]);
+        float sum[1] = {dot8(f, f)};
         norm_sum<1, CLUSTER>(sum, at, red, peer, turn);
-        const float inv = norm_inv(sum[0], d, c.D.eps_post);
-#pragma unroll
-        for (int i = 0; i < NORM_VALUES; i++) p[i] = __fmul_rn(p[i], inv);
+        s = __fmul_rn(s, norm_inv(sum[0], c.inv_d, c.D.eps_post));
       }
-#pragma unroll
-      for (int i = 0; i < NORM_VALUES; i++) r[i] = __fmaf_rn(__fmul_rn(p[i], wp[i]), s, r[i]);
+      r = fma8(f * wp, s, r);
     }
-    if (c.r) NormRow<E, V>::store(c.r, (size_t)t * c.D.r_stride, at, d, r);
+    if (has_r) NormRow<E, V>::store(c.r, norm_row(t, c.D.r_stride), at, d, r);
     if (pre) {
-      sum[0] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NORM_VALUES; i++) sum[0] = __fmaf_rn(r[i], r[i], sum[0]);
+      float sum[1] = {dot8(r, r)};
       norm_sum<1, CLUSTER>(sum, at, red, peer, turn);
-      const float inv = norm_inv(sum[0], d, c.D.eps_pre);
-#pragma unroll
-      for (int i = 0; i < NORM_VALUES; i++) p[i] = __fmul_rn(__fmul_rn(r[i], inv), wn[i]);
-      NormRow<E, V>::store(c.n, (size_t)t * c.D.n_stride, at, d, p);
+      NormRow<E, V>::store(c.n, norm_row(t, c.D.n_stride), at, d, r * wn * norm_inv(sum[0], c.inv_d, c.D.eps_pre));
     }
   }
   if constexpr (CLUSTER) cg::this_cluster().sync();  // no CTA leaves while another may still write its sums here
 }
 
-// Each group adds up the weights' gradients of its rows in registers; a CTA adds its groups and leaves a row of sums in
-// parts[kind][CTA][d], which k_norm_sum_parts adds up. No atomics.
-template <typename E, typename W, int V, bool CLUSTER>
-__global__ void __launch_bounds__(1024) k_block_norm_grad(NormCall c, int tpr, int rpb, int cl) {
+// Three sweeps over a row's values: the sums of both norms; D, dx, the weights' gradients and the sum of v f; df. The values
+// are read again from the ring each time and the weights lie beside it (f32, the thread's own columns): the 16 sums of the
+// weights' gradients fill the registers. A CTA adds up its groups and leaves a row of sums in parts[kind][CTA][d], which
+// k_norm_sum_parts adds up. No atomics.
+template <typename E, typename W, int V, bool CLUSTER, bool RING, NormMode MODE>
+__global__ void __launch_bounds__(NORM_GRAD_THREADS) k_block_norm_grad(NormCall c, int tpr, int rpb, int cl, int stages) {
   pm_pdl();
-  extern __shared__ float fold[];  // [threads][8]
-  __shared__ float red3[2][32][3], peer3[2][8][3], red[2][32][1], peer[2][8][1];
+  extern __shared__ uint4 slots[];
+  __shared__ NormRed<3> red3;
+  __shared__ NormPeer<3> peer3;
+  __shared__ NormRed<1> red;
+  __shared__ NormPeer<1> peer;
   const NormPlace at = norm_place<CLUSTER>(tpr, cl, V);
   const int d = c.D.d, n_parts = (int)(gridDim.x / at.cl), part = (int)(blockIdx.x / at.cl), groups = n_parts * rpb;
-  const bool post = c.D.flags & PM_NORM_POST, pre = c.D.flags & PM_NORM_PRE;
-  const bool channel = c.D.gate == PM_NORM_GATE_CHANNEL;
-  float a_pre[NORM_VALUES] = {}, a_post[NORM_VALUES] = {}, a_gate[NORM_VALUES] = {};
-  float wp[NORM_VALUES], wn[NORM_VALUES], wg[NORM_VALUES];
-  norm_weights<W, V>(wp, post ? c.w_post : nullptr, c.D.offset_post, at, d);
-  norm_weights<W, V>(wn, pre ? c.w_pre : nullptr, c.D.offset_pre, at, d);
-  norm_weights<W, V>(wg, channel ? c.gate : nullptr, 0.0f, at, d);
-  int turn3 = 0, turn = 0;
-  for (int t = part * rpb + at.group; t < c.T; t += groups) {
-    NormRow<E, V> rr, fr, drr, dnr;
-    float r[NORM_VALUES], f[NORM_VALUES], D[NORM_VALUES], u[NORM_VALUES];
-    const size_t at_r = (size_t)t * c.D.r_stride, at_f = (size_t)t * c.D.f_stride;
-    if (pre) {
-      rr.load(c.x, at_r, at, d);
-      dnr.load(c.dn, (size_t)t * c.D.n_stride, at, d);
+  constexpr bool ANY = MODE == NORM_ANY;
+  const bool post = ANY ? c.D.flags & PM_NORM_POST : MODE == NORM_SANDWICH, pre = ANY ? c.D.flags & PM_NORM_PRE : true;
+  const bool channel = c.D.gate == PM_NORM_GATE_CHANNEL, token = MODE != NORM_BEFORE && c.D.gate == PM_NORM_GATE_TOKEN;
+  const bool use_f = ANY ? post || channel || token : MODE == NORM_SANDWICH;  // (plain: df = beta D)
+  const bool has_dr = ANY ? c.dr != nullptr : true, has_dx = ANY ? c.dx != nullptr : true, has_df = ANY ? c.df != nullptr : true;
+  const NormSlots own = norm_slots(slots);
+  // slots: the pre weight, post weight times the channel's gate, the ring
+  const int i_f = pre ? 2 : 0, i_dr = i_f + (use_f ? 1 : 0);
+  const NormRing<E, V, RING> ring = {own, 4, i_dr + (has_dr ? 1 : 0), stages};
+  const int t0 = part * rpb + at.group;
+  auto copy = [&](int stage, int t) {
+    if (t < c.T) {
+      uint32_t row = ring.row(stage);
+      if (pre) {
+        ring.copy(row, 0, c.x, norm_row(t, c.D.r_stride), at, d);
+        ring.copy(row, 1, c.dn, norm_row(t, c.D.n_stride), at, d);
+      }
+      if (use_f) ring.copy(row, i_f, c.f, norm_row(t, c.D.f_stride), at, d);
+      if (has_dr) ring.copy(row, i_dr, c.dr, norm_row(t, c.D.r_stride), at, d);
     }
-    if (c.f) fr.load(c.f, at_f, at, d);
-    if (c.dr) {
-      drr.load(c.dr, at_r, at, d);
-      drr.widen(D);
-    } else {
-#pragma unroll
-      for (int i = 0; i < NORM_VALUES; i++) D[i] = 0.0f;
-    }
+    ring.commit();
+  };
+  ring.clear();
+  if constexpr (RING)
+    for (int s = 0; s < stages; s++) copy(s, t0 + s * groups);
+  own.put8(0, norm_weights<W, V>(pre ? c.w_pre : nullptr, c.D.offset_pre, at, d));
+  own.put8(2, norm_weights<W, V>(post ? c.w_post : nullptr, c.D.offset_post, at, d) * norm_weights<W, V>(channel ? c.gate : nullptr, 0.0f, at, d));
+  F8 a_pre = F8::all(0.0f), a_dk = F8::all(0.0f);
+  int turn3 = 0, turn = 0, stage = 0;
+  for (int t = t0; t < c.T; t += groups) {
+    const size_t at_r = norm_row(t, c.D.r_stride), at_f = norm_row(t, c.D.f_stride), at_n = norm_row(t, c.D.n_stride);
+    const uint32_t row = ring.row(stage);
+    NormRow<E, V> raw, fr;
     float sum[3] = {0.0f, 0.0f, 0.0f};
+    ring.wait();
     if (pre) {
-      rr.widen(r);
-      dnr.widen(u);
-#pragma unroll
-      for (int i = 0; i < NORM_VALUES; i++) {
-        sum[0] = __fmaf_rn(r[i], r[i], sum[0]);
-        sum[1] = __fmaf_rn(__fmul_rn(u[i], wn[i]), r[i], sum[1]);
-      }
+      ring.get(raw, row, 0, c.x, at_r, at, d);
+      const F8 r = raw.widen();
+      ring.get(raw, row, 1, c.dn, at_n, at, d);
+      sum[0] = dot8(r, r);
+      sum[1] = dot8(raw.widen() * own.get8(0), r);
     }
-    if (c.f) {
-      fr.widen(f);
-      if (post) {
-#pragma unroll
-        for (int i = 0; i < NORM_VALUES; i++) sum[2] = __fmaf_rn(f[i], f[i], sum[2]);
-      }
+    if (use_f) ring.get(fr, row, i_f, c.f, at_f, at, d);
+    if (post) {
+      const F8 f = fr.widen();
+      sum[2] = dot8(f, f);
     }
     if (pre || post) norm_sum<3, CLUSTER>(sum, at, red3, peer3, turn3);
+    F8 D = F8::all(0.0f);
+    if (has_dr) {
+      ring.get(raw, row, i_dr, c.dr, at_r, at, d);
+      D = raw.widen();
+    }
     if (pre) {
-      const float s2 = norm_inv(sum[0], d, c.D.eps_pre);
-      const float m = __fmul_rn(__fmul_rn(s2, s2), __fdiv_rn(sum[1], (float)d));
-#pragma unroll
-      for (int i = 0; i < NORM_VALUES; i++) {
-        a_pre[i] = __fmaf_rn(u[i], __fmul_rn(r[i], s2), a_pre[i]);
-        D[i] = __fmaf_rn(s2, __fmaf_rn(-r[i], m, __fmul_rn(u[i], wn[i])), D[i]);
+      const float s2 = norm_inv(sum[0], c.inv_d, c.D.eps_pre);
+      const float m = __fmul_rn(__fmul_rn(s2, s2), __fmul_rn(sum[1], c.inv_d));
+      ring.get(raw, row, 0, c.x, at_r, at, d);
+      const F8 r = raw.widen();
+      ring.get(raw, row, 1, c.dn, at_n, at, d);
+      const F8 dn = raw.widen();
+      a_pre = fma8(dn, r * s2, a_pre);
+      D = fma8(fma8(r, -m, dn * own.get8(0)), s2, D);
+    }
+    if constexpr (RING) {  // (f is in registers)
+      copy(stage, t + stages * groups);
+      stage = stage + 1 == stages ? 0 : stage + 1;
+    }
+    if (has_dx) NormRow<E, V>::store(c.dx, norm_row(t, c.D.x_stride), at, d, D * c.D.alpha);
+    if (!use_f && !has_df) continue;
+    // D becomes beta g D, g of the token, then beta g D (o1 + w_post) of either gate; k = f s1
+    const float gt = MODE == NORM_BEFORE ? 1.0f : norm_token_gate<W>(c, t);
+    float s1 = 1.0f, mean = 0.0f;
+    if (use_f) {
+      if (post) s1 = norm_inv(sum[2], c.inv_d, c.D.eps_post);
+      const F8 k = fr.widen() * s1;
+      D = D * c.D.beta;
+      if (post || channel) a_dk = fma8(D * gt, k, a_dk);
+      D = D * own.get8(2);
+      if (post || token) {
+        float dot[1] = {dot8(D, k)};
+        norm_sum<1, CLUSTER>(dot, at, red, peer, turn);
+        if (token && c.dgate && at.rank == 0 && at.warp == 0 && at.lane == 0) c.dgate[t] = dot[0];
+        mean = __fmul_rn(__fmul_rn(dot[0], gt), c.inv_d);
       }
+      D = D * gt;
+    } else {
+      D = D * c.D.beta;
     }
-    if (c.dx) {
-#pragma unroll
-      for (int i = 0; i < NORM_VALUES; i++) u[i] = __fmul_rn(c.D.alpha, D[i]);
-      NormRow<E, V>::store(c.dx, (size_t)t * c.D.x_stride, at, d, u);
+    if (has_df) {
+      if (post) D = fma8(fr.widen() * s1, -mean, D) * s1;
+      NormRow<E, V>::store(c.df, at_f, at, d, D);
     }
-    if (!c.f) continue;
-    const float s1 = post ? norm_inv(sum[2], d, c.D.eps_post) : 1.0f;
-    const float gt = norm_token_gate<W>(c, t);
-    // u = beta D, q = beta g D (g of the channel; the token's gate is one factor of the row)
-    float dot[1] = {0.0f};
-#pragma unroll
-    for (int i = 0; i < NORM_VALUES; i++) {
-      u[i] = __fmul_rn(c.D.beta, D[i]);
-      const float pw = __fmul_rn(__fmul_rn(f[i], s1), wp[i]);
-      if (channel) a_gate[i] = __fmaf_rn(u[i], pw, a_gate[i]);
-      u[i] = __fmul_rn(u[i], wg[i]);
-      dot[0] = __fmaf_rn(u[i], pw, dot[0]);
-      a_post[i] = __fmaf_rn(__fmul_rn(u[i], gt), __fmul_rn(f[i], s1), a_post[i]);
-    }
-    if (post || c.D.gate == PM_NORM_GATE_TOKEN) norm_sum<1, CLUSTER>(dot, at, red, peer, turn);  // sum of u (f s1 w) over the row
-    if (c.D.gate == PM_NORM_GATE_TOKEN && c.dgate && at.rank == 0 && at.warp == 0 && at.lane == 0) c.dgate[t] = dot[0];
-    const float m = __fdiv_rn(__fmul_rn(dot[0], gt), (float)d);  // mean(v f) s1
-#pragma unroll
-    for (int i = 0; i < NORM_VALUES; i++) {
-      const float q = __fmul_rn(u[i], gt);
-      f[i] = post ? __fmul_rn(s1, __fmaf_rn(-__fmul_rn(f[i], s1), m, __fmul_rn(q, wp[i]))) : q;
-    }
-    if (c.df) NormRow<E, V>::store(c.df, at_f, at, d, f);
   }
-  // the CTA's groups, kind by kind, columns of a thread as it holds them
+  // The CTA's groups, kind by kind, columns of a thread as it holds them. With K = sum over t of beta g_t D k, dw_post is K times
+  // the channel's gate and the channel's dgate is K times the post weight.
+  if constexpr (RING) asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-  for (int kind = 0; kind < 3; kind++) {
-    const bool on = kind == 0 ? pre && c.dw_pre : kind == 1 ? post && c.dw_post && c.f : channel && c.dgate;
+  for (int kind = 0; kind < 2; kind++) {
+    const bool on = kind == 0 ? pre && c.dw_pre : (post && c.dw_post) || (channel && c.dgate);
     if (!on) continue;
-    float *a = kind == 0 ? a_pre : kind == 1 ? a_post : a_gate;
+    F8 sums = kind == 0 ? a_pre : a_dk;
     if (rpb > 1) {
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NORM_VALUES; i++) fold[i * blockDim.x + threadIdx.x] = a[i];
+      own.put8(0, sums);  // (the weights have served)
       __syncthreads();
       if (at.group == 0)
-        for (int g = 1; g < rpb; g++)
-#pragma unroll
-          for (int i = 0; i < NORM_VALUES; i++) a[i] = __fadd_rn(a[i], fold[i * blockDim.x + g * tpr + threadIdx.x]);
+        for (int g = 1; g < rpb; g++) sums = sums + NormSlots{own.mine + g * tpr * 16, own.pitch}.get8(0);
     }
-    if (at.group == 0) {
-      float *to = c.parts + ((size_t)kind * n_parts + part) * d;
+    auto leave = [&](int which, const F8 &s) {
+      float a[NORM_VALUES];
+#pragma unroll
+      for (int i = 0; i < 4; i++) pm_unpack2(s.p[i], a[2 * i], a[2 * i + 1]);
+      float *to = c.parts + ((size_t)which * n_parts + part) * d;
 #pragma unroll
       for (int j = 0; j < NORM_VALUES / V; j++) {
         const int col = at.col0 + j * tpr * at.cl * V;
@@ -317,6 +440,12 @@ __global__ void __launch_bounds__(1024) k_block_norm_grad(NormCall c, int tpr, i
         for (int i = 0; i < V; i++)
           if (col + i < d) to[col + i] = a[j * V + i];
       }
+    };
+    if (at.group) continue;
+    if (kind == 0) leave(0, sums);
+    else {
+      if (post && c.dw_post) leave(1, channel ? sums * norm_weights<W, V>(c.gate, 0.0f, at, d) : sums);
+      if (channel && c.dgate) leave(2, post ? sums * norm_weights<W, V>(c.w_post, c.D.offset_post, at, d) : sums);
     }
   }
   if constexpr (CLUSTER) cg::this_cluster().sync();
@@ -347,20 +476,31 @@ __global__ void __launch_bounds__(256) k_norm_sum_parts(const float *__restrict_
 // ---------------------------------------------------------------------------
 // launchers
 // ---------------------------------------------------------------------------
-// CTAs (clusters) of a call: rows there are, at most what 1,024 threads an SM make resident
+// CTAs (clusters) of a call: rows there are, at most what is resident
 static int norm_parts(const NormShape &s, int T, int n_sm) {
-  const int per_sm = 1024 / (s.tpr * s.rpb);
-  const int most = s.cl > 1 ? n_sm / s.cl : n_sm * (per_sm > 0 ? per_sm : 1);
+  const int most = s.cl > 1 ? n_sm / s.cl : n_sm * s.per_sm;
   const int need = (T + s.rpb - 1) / s.rpb;
   return need < most ? need : most;
 }
-size_t norm_parts_floats(const pm_norm_desc &D, int T, int n_sm) { return (size_t)3 * norm_parts(norm_shape(D.d), T, n_sm) * D.d; }
+size_t norm_parts_floats(const pm_norm_desc &D, int T, int n_sm) { return (size_t)3 * norm_parts(norm_shape(D.d, NORM_GRAD_THREADS), T, n_sm) * D.d; }
+
+// the rows of `row` slots that fit into a ring beside `fixed` slots a thread, 3 at most; fewer CTAs on an SM where two would not fit
+static void norm_ring(NormShape &s, int fixed, int row) {
+  auto fit = [&](int per_sm) { return ((NORM_SMEM / per_sm - NORM_SMEM_CTA) / (s.threads() * 16) - fixed) / row; };
+  while (s.per_sm > 1 && fit(s.per_sm) < 2) s.per_sm--;
+  const int n = fit(s.per_sm);
+  s.stages = n > 3 ? 3 : n < 1 ? 1 : n;
+  s.slots = fixed + s.stages * row;
+}
 
 template <typename... P>
-static cudaError_t norm_launch(const Launch &L, void (*kern)(P...), int parts, const NormShape &s, size_t smem, NormCall c) {
+static cudaError_t norm_launch(const Launch &L, SmemOptIn &opt, void (*kern)(P...), int parts, const NormShape &s, NormCall c) {
+  const size_t smem = (size_t)s.threads() * s.slots * 16;
+  const cudaError_t e = smem_optin(opt, kern, smem);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(parts * s.cl);
-  cfg.blockDim = dim3(s.tpr * s.rpb);
+  cfg.blockDim = dim3(s.threads());
   cfg.dynamicSmemBytes = smem;
   cfg.stream = L.stream;
   cudaLaunchAttribute at[2];
@@ -372,23 +512,54 @@ static cudaError_t norm_launch(const Launch &L, void (*kern)(P...), int parts, c
   cfg.attrs = at;
   cfg.numAttrs = s.cl > 1 ? 2 : 1;
   if (L.count) ++*L.count;
-  return cudaLaunchKernelEx(&cfg, kern, c, s.tpr, s.rpb, s.cl);
+  return cudaLaunchKernelEx(&cfg, kern, c, s.tpr, s.rpb, s.cl, s.stages);
+}
+template <typename E, typename W, int V, bool RING, NormMode MODE, bool GRAD>
+static cudaError_t norm_go(const Launch &L, int parts, const NormShape &s, const NormCall &c) {
+  static SmemOptIn one, many;
+  if constexpr (GRAD)
+    return s.cl > 1 ? norm_launch(L, many, k_block_norm_grad<E, W, V, true, RING, MODE>, parts, s, c)
+                    : norm_launch(L, one, k_block_norm_grad<E, W, V, false, RING, MODE>, parts, s, c);
+  else
+    return s.cl > 1 ? norm_launch(L, many, k_block_norm<E, W, V, true, RING, MODE>, parts, s, c)
+                    : norm_launch(L, one, k_block_norm<E, W, V, false, RING, MODE>, parts, s, c);
+}
+// the kernels of 16-byte words that go by what the call has
+template <typename E, typename W, int V, bool GRAD>
+static cudaError_t norm_go_mode(const Launch &L, int parts, const NormShape &s, const NormCall &c) {
+  const bool all = GRAD ? c.dr && c.dx && c.df : c.x && c.f && c.r;
+  const bool post = c.D.flags & PM_NORM_POST, pre = c.D.flags & PM_NORM_PRE;
+  if (all && pre && post) return norm_go<E, W, V, true, NORM_SANDWICH, GRAD>(L, parts, s, c);
+  if (all && pre && c.D.gate == PM_NORM_GATE_NONE) return norm_go<E, W, V, true, NORM_BEFORE, GRAD>(L, parts, s, c);
+  return norm_go<E, W, V, true, NORM_ANY, GRAD>(L, parts, s, c);
 }
 
 template <typename E, typename W, int V> static cudaError_t norm_forward(const Launch &L, const NormCall &c) {
-  const NormShape s = norm_shape(c.D.d);
-  const int parts = norm_parts(s, c.T, L.n_sm);
-  return s.cl > 1 ? norm_launch(L, k_block_norm<E, W, V, true>, parts, s, 0, c) : norm_launch(L, k_block_norm<E, W, V, false>, parts, s, 0, c);
+  NormShape s = norm_shape(c.D.d, NORM_THREADS);
+  // a ring where a group has a second row to fetch
+  if constexpr (V > 1) {
+    if (c.T > norm_parts(s, c.T, L.n_sm) * s.rpb) {
+      norm_ring(s, 0, ((c.x ? 1 : 0) + (c.f ? 1 : 0)) * NORM_VALUES / V);
+      return norm_go_mode<E, W, V, false>(L, norm_parts(s, c.T, L.n_sm), s, c);
+    }
+  }
+  return norm_go<E, W, V, false, NORM_ANY, false>(L, norm_parts(s, c.T, L.n_sm), s, c);
 }
 template <typename E, typename W, int V> static cudaError_t norm_backward(const Launch &L, const NormCall &c) {
-  const NormShape s = norm_shape(c.D.d);
-  const int parts = norm_parts(s, c.T, L.n_sm);
-  const size_t fold = s.rpb > 1 ? (size_t)s.tpr * s.rpb * NORM_VALUES * sizeof(float) : 0;  // 8 KB: rpb is 1 from 256 threads on
-  cudaError_t e = cudaSuccess;  // (no rows: the sums alone, zeros)
-  if (parts) e = s.cl > 1 ? norm_launch(L, k_block_norm_grad<E, W, V, true>, parts, s, fold, c)
-                          : norm_launch(L, k_block_norm_grad<E, W, V, false>, parts, s, fold, c);
-  if (e != cudaSuccess) return e;
+  NormShape s = norm_shape(c.D.d, NORM_GRAD_THREADS);
+  int parts = 0;
   float *channel = c.D.gate == PM_NORM_GATE_CHANNEL ? c.dgate : nullptr;
+  if (c.T) {  // (no rows: the sums alone, zeros)
+    const bool post = c.D.flags & PM_NORM_POST, pre = c.D.flags & PM_NORM_PRE, gate = c.D.gate != PM_NORM_GATE_NONE;
+    const int row = ((pre ? 2 : 0) + (post || gate ? 1 : 0) + (c.dr ? 1 : 0)) * NORM_VALUES / V;
+    s.slots = 4;
+    if (V > 1 && row) norm_ring(s, 4, row);
+    parts = norm_parts(s, c.T, L.n_sm);
+    cudaError_t e;
+    if constexpr (V > 1) e = norm_go_mode<E, W, V, true>(L, parts, s, c);
+    else e = norm_go<E, W, V, false, NORM_ANY, true>(L, parts, s, c);
+    if (e != cudaSuccess) return e;
+  }
   if (!c.dw_pre && !c.dw_post && !channel) return cudaSuccess;
   return pm_launch(L, k_norm_sum_parts, dim3((c.D.d + 31) / 32, 3), 256, 0, (const float *)c.parts, parts, c.D.d, c.dw_pre, c.dw_post, channel);
 }

@@ -6,6 +6,7 @@
 struct NormCall {
   pm_norm_desc D;  // strides filled in
   int T;
+  float inv_d;     // 1 / d
   bool vec;        // every row of every stream and every weight starts on 16 bytes, rows are whole 16-byte words
   const void *x, *f, *w_post, *gate, *w_pre;  // x: of the gradient, the stream behind the block
   // forward

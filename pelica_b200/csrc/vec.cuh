@@ -42,14 +42,78 @@ template <typename E, int V> __device__ __forceinline__ void pm_store(E *p, cons
     *p = r.v[0];
   }
 }
-template <typename E, int V> __device__ __forceinline__ void pm_widen(const Raw<E, V> &r, float (&f)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; i++) f[i] = pm_to_f32(r.v[i]);
+// two neighbouring values as one f32x2 register pair, and back with the one rounding of a result (to nearest)
+__device__ __forceinline__ uint64_t pm_widen2(const float *v) { return pm_pack2(v[0], v[1]); }
+__device__ __forceinline__ uint64_t pm_widen2(const __half *v) {
+  const float2 f = __half22float2(*(const __half2 *)v);
+  return pm_pack2(f.x, f.y);
 }
-// to the stream's type: the one rounding of a result, to nearest
+__device__ __forceinline__ uint64_t pm_widen2(const __nv_bfloat16 *v) {  // the upper half of an f32 each
+  const uint32_t w = *(const uint32_t *)v;
+  return pm_pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ void pm_narrow2(float *o, float a, float b) { o[0] = a, o[1] = b; }
+__device__ __forceinline__ void pm_narrow2(__half *o, float a, float b) { *(__half2 *)o = __floats2half2_rn(a, b); }
+__device__ __forceinline__ void pm_narrow2(__nv_bfloat16 *o, float a, float b) { *(__nv_bfloat162 *)o = __floats2bfloat162_rn(a, b); }
+
+template <typename E, int V> __device__ __forceinline__ void pm_widen(const Raw<E, V> &r, float (&f)[V]) {
+  if constexpr (V == 1) {
+    f[0] = pm_to_f32(r.v[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) pm_unpack2(pm_widen2(&r.v[i]), f[i], f[i + 1]);
+  }
+}
 template <typename E, int V> __device__ __forceinline__ Raw<E, V> pm_narrow(const float (&f)[V]) {
   Raw<E, V> r;
+  if constexpr (V == 1) {
+    r.v[0] = pm_from_f32<E>(f[0]);
+  } else {
 #pragma unroll
-  for (int i = 0; i < V; i++) r.v[i] = pm_from_f32<E>(f[i]);
+    for (int i = 0; i < V; i += 2) pm_narrow2(&r.v[i], f[i], f[i + 1]);
+  }
   return r;
+}
+
+// eight f32 values as four pairs: one instruction works on a pair (each value rounded as by the scalar one)
+__device__ __forceinline__ uint64_t pm_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pm_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+struct F8 {
+  uint64_t p[4];
+  __device__ __forceinline__ static F8 all(float v) {
+    const uint64_t b = pm_pack2(v, v);
+    return {{b, b, b, b}};
+  }
+  __device__ __forceinline__ float sum() const {
+    const uint64_t a = pm_add2(pm_add2(p[0], p[1]), pm_add2(p[2], p[3]));
+    float x, y;
+    pm_unpack2(a, x, y);
+    return __fadd_rn(x, y);
+  }
+};
+__device__ __forceinline__ F8 operator*(const F8 &a, const F8 &b) {
+  return {{pm_mul2(a.p[0], b.p[0]), pm_mul2(a.p[1], b.p[1]), pm_mul2(a.p[2], b.p[2]), pm_mul2(a.p[3], b.p[3])}};
+}
+__device__ __forceinline__ F8 operator*(const F8 &a, float s) { return a * F8::all(s); }
+__device__ __forceinline__ F8 operator+(const F8 &a, const F8 &b) {
+  return {{pm_add2(a.p[0], b.p[0]), pm_add2(a.p[1], b.p[1]), pm_add2(a.p[2], b.p[2]), pm_add2(a.p[3], b.p[3])}};
+}
+__device__ __forceinline__ F8 fma8(const F8 &a, const F8 &b, const F8 &c) {
+  return {{pm_fma2(a.p[0], b.p[0], c.p[0]), pm_fma2(a.p[1], b.p[1], c.p[1]), pm_fma2(a.p[2], b.p[2], c.p[2]), pm_fma2(a.p[3], b.p[3], c.p[3])}};
+}
+__device__ __forceinline__ F8 fma8(const F8 &a, float s, const F8 &c) { return fma8(a, F8::all(s), c); }
+// the sum of a b over the eight
+__device__ __forceinline__ float dot8(const F8 &a, const F8 &b) {
+  const uint64_t s = pm_fma2(a.p[3], b.p[3], pm_fma2(a.p[2], b.p[2], pm_fma2(a.p[1], b.p[1], pm_mul2(a.p[0], b.p[0]))));
+  float x, y;
+  pm_unpack2(s, x, y);
+  return __fadd_rn(x, y);
 }
