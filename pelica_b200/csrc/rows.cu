@@ -161,38 +161,61 @@ __global__ void __launch_bounds__(256) k_rows_dispatch_small(RowsCall c, const u
 // ---------------------------------------------------------------------------
 // the plan of many pairs
 // ---------------------------------------------------------------------------
-// One cluster of 8 CTAs x 32 warps; a warp owns a run of pairs. First pass: a pair's rank within its warp (match.any: the
-// lanes with the same expert) and the warp's counts, u16 in shared memory. Then sums over a CTA's warps, over the CTAs
-// through distributed shared memory, over the experts. Second pass: positions. No scratch in global memory, so a recorded
-// graph holds no pointer of the library's; a pair's rank waits for the second pass in its place of `pos`.
+// Clusters of 8 CTAs x 32 warps, each of which places a run of 8,192 pairs times `steps`; a warp owns 32 pairs a step. A pair's
+// rank within its warp (match.any: the lanes with the same expert) comes from the warp's counts, u16 in shared memory; then
+// sums over a CTA's warps and over the CTAs through distributed shared memory. A cluster counts the pairs in front of its run
+// and behind it itself - no ranks, so shared-memory additions do - instead of waiting for the other clusters: nothing is
+// exchanged in global memory, and a recorded graph holds no pointer of the library's. 131,072 pairs: 25 us in one
+// cluster, whose 8 SMs wait for match.any (votes bit by bit: as long).
 #define SORT_CTAS 8
 #define SORT_WARPS 32
-__global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_WARPS * 32)
-    k_rows_sort(RowsCall c, const uint32_t *__restrict__ ids, const float *__restrict__ w) {
+#define SORT_THREADS (SORT_WARPS * 32)
+#define SORT_RUN (SORT_CTAS * SORT_THREADS)  // pairs of a cluster's step
+#define SORT_CLUSTERS 8
+#define SORT_STEPS (PM_MAX_TOKENS * PM_MAX_TOPK / (SORT_RUN * SORT_CLUSTERS))
+__global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS)
+    k_rows_sort(RowsCall c, uint32_t steps, const uint32_t *__restrict__ ids, const float *__restrict__ w) {
   pm_pdl();
   __shared__ uint16_t hist[SORT_WARPS][PM_MAX_EXPERTS];
-  __shared__ uint32_t total[PM_MAX_EXPERTS], cnt[PM_MAX_EXPERTS], off[PM_MAX_EXPERTS + 1], part[8];
+  __shared__ uint32_t ours[PM_MAX_EXPERTS], front[PM_MAX_EXPERTS], behind[PM_MAX_EXPERTS];
+  __shared__ uint32_t cnt[PM_MAX_EXPERTS], off[PM_MAX_EXPERTS + 1], part[8];
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t rank = cluster.block_rank(), P = (uint32_t)c.T * c.D.top_k;
-  // a run of 32 * steps pairs a warp
-  const uint32_t steps = (P + SORT_CTAS * SORT_WARPS * 32 - 1) / (SORT_CTAS * SORT_WARPS * 32);
-  const uint32_t first = (rank * SORT_WARPS + warp) * steps * 32 + lane;
-  for (int i = tid; i < SORT_WARPS * PM_MAX_EXPERTS / 2; i += SORT_WARPS * 32) ((uint32_t *)hist)[i] = 0;
+  const uint32_t rank = cluster.block_rank(), run = blockIdx.x / SORT_CTAS, P = (uint32_t)c.T * c.D.top_k;
+  const uint32_t begin = run * steps * SORT_RUN, end = min(begin + steps * SORT_RUN, P);
+  const uint32_t first = begin + (rank * SORT_WARPS + warp) * steps * 32 + lane;
+  uint32_t mine[SORT_STEPS];  // ids, then expert << 16 | rank
+#pragma unroll
+  for (int s = 0; s < SORT_STEPS; s++) mine[s] = s < (int)steps && first + s * 32 < P ? ids[first + s * 32] : PM_ROWS_NONE;
+  for (int i = tid; i < SORT_WARPS * PM_MAX_EXPERTS / 2; i += SORT_THREADS) ((uint32_t *)hist)[i] = 0;
+  if (tid < PM_MAX_EXPERTS) front[tid] = behind[tid] = 0;
   __syncthreads();
-  for (uint32_t s = 0; s < steps; s++) {
-    const uint32_t p = first + s * 32, e = p < P ? rows_local(c, ids[p]) : ROWS_NO_EXPERT;
-    const uint32_t same = __match_any_sync(PM_FULL, e);
-    const uint32_t before = __popc(same & ((1u << lane) - 1));
+  for (uint32_t p0 = rank * SORT_THREADS + tid; p0 < P; p0 += 4 * SORT_RUN) {
+    uint32_t id[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t p = p0 + i * SORT_RUN;
+      id[i] = p < P && (p < begin || p >= end) ? ids[p] : PM_ROWS_NONE;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t e = id[i] - (uint32_t)c.D.first_expert;  // (an id that no expert has is its own cluster's to report)
+      if (id[i] < (uint32_t)c.D.n_exp && e < (uint32_t)c.D.n_local) atomicAdd(p0 + i * SORT_RUN < begin ? &front[e] : &behind[e], 1u);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < SORT_STEPS; s++) {
+    if (s >= (int)steps) break;
+    const uint32_t e = rows_local(c, mine[s]), same = __match_any_sync(PM_FULL, e), before = __popc(same & ((1u << lane) - 1));
     uint32_t have = 0;
     if (e != ROWS_NO_EXPERT) have = hist[warp][e];
     __syncwarp();
     if (e != ROWS_NO_EXPERT && before == 0) hist[warp][e] = (uint16_t)(have + __popc(same));
     __syncwarp();
-    if (p < P) c.pl.pos[p] = e != ROWS_NO_EXPERT ? have + before : PM_ROWS_NONE;
+    mine[s] = e << 16 | (have + before);
   }
   __syncthreads();
-  if (tid < PM_MAX_EXPERTS) {  // the warps' counts become what lies before each warp (a CTA has 32,768 pairs at most)
+  if (tid < PM_MAX_EXPERTS) {  // the warps' counts become what lies before each warp (a CTA has 4,096 pairs at most)
     uint32_t sum = 0;
 #pragma unroll 8
     for (int i = 0; i < SORT_WARPS; i++) {
@@ -200,178 +223,148 @@ __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_WARPS *
       hist[i][tid] = (uint16_t)sum;
       sum += n;
     }
-    total[tid] = sum;
+    ours[tid] = sum;
   }
   cluster.sync();
-  uint32_t ahead = 0;  // pairs of expert tid in the CTAs before this one
+  uint32_t ahead = 0;  // pairs of expert tid in front of this CTA's
   if (tid < PM_MAX_EXPERTS) {
     uint32_t all = 0;
 #pragma unroll
     for (int i = 0; i < SORT_CTAS; i++) {
-      const uint32_t n = cluster.map_shared_rank(total, i)[tid];
-      if (i < (int)rank) ahead += n;
-      all += n;
+      const uint32_t n = cluster.map_shared_rank(ours, i)[tid], f = cluster.map_shared_rank(front, i)[tid];
+      ahead += f + (i < (int)rank ? n : 0);
+      all += f + n + cluster.map_shared_rank(behind, i)[tid];
     }
     cnt[tid] = all;
   }
   cluster.sync();  // nobody reads another CTA's counts any more
   rows_scan(cnt, c.D.align, off, part);
-  if (tid < PM_MAX_EXPERTS) total[tid] = off[tid] + ahead;
-  if (rank == 0) {
-    for (int e = tid; e < c.D.n_local; e += SORT_WARPS * 32) {
+  if (tid < PM_MAX_EXPERTS) ours[tid] = off[tid] + ahead;
+  if (blockIdx.x == 0) {
+    for (int e = tid; e < c.D.n_local; e += SORT_THREADS) {
       c.pl.offset[e] = off[e];
       c.pl.count[e] = cnt[e];
     }
     if (tid == 0) c.pl.offset[c.D.n_local] = off[c.D.n_local];
   }
   __syncthreads();
-  for (uint32_t s = 0; s < steps; s++) {
-    const uint32_t p = first + s * 32;
-    if (p >= P) break;
-    const uint32_t r = c.pl.pos[p];
-    if (r == PM_ROWS_NONE) continue;
-    const uint32_t e = rows_local(c, ids[p]);
-    rows_write_pair(c, w, p, e + (uint32_t)c.D.first_expert, total[e] + hist[warp][e] + r);
+#pragma unroll
+  for (int s = 0; s < SORT_STEPS; s++) {
+    const uint32_t p = first + s * 32, e = mine[s] >> 16;
+    if (s >= (int)steps || p >= P) break;
+    rows_write_pair(c, w, p, e + (uint32_t)c.D.first_expert, e == ROWS_NO_EXPERT ? PM_ROWS_NONE : ours[e] + hist[warp][e] + (mine[s] & 0xffffu));
   }
   if (c.D.align > 1 && (c.pl.row_pair || c.pl.row_expert || c.pl.row_weight))
-    for (uint32_t e = rank * SORT_WARPS + warp; e < (uint32_t)c.D.n_local; e += SORT_CTAS * SORT_WARPS)
+    for (uint32_t e = blockIdx.x * SORT_WARPS + warp; e < (uint32_t)c.D.n_local; e += gridDim.x * SORT_WARPS)
       for (uint32_t r = off[e] + cnt[e] + lane; r < off[e + 1]; r += 32) rows_write_pad(c, e, r);
 }
 
 // ---------------------------------------------------------------------------
-// copies and sums without a dot product: a thread a vector of a token
+// rows out and rows back: G threads a token
 // ---------------------------------------------------------------------------
-// Grid: CTAs of 256 vectors, behind them (SPREAD) one CTA an expert for the padding of its group.
-template <typename E, int V>
-__global__ void __launch_bounds__(256) k_rows_spread(RowsCall c, uint32_t copy_ctas, const float *__restrict__ w, const E *__restrict__ src,
-                                                     E *__restrict__ out) {
-  pm_pdl();
-  const uint32_t dv = (uint32_t)c.D.d / V, K = c.D.top_k;
-  if (blockIdx.x >= copy_ctas) {
-    const uint32_t e = blockIdx.x - copy_ctas;
-    const uint32_t from = c.pl.offset[e] + c.pl.count[e], to = c.pl.offset[e + 1];
-    rows_zero<E, V>(c, out, from, (uint32_t)min((int64_t)to, c.pl.max_rows));
-    return;
-  }
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x, t = i / dv, v = i - t * dv;
-  if (t >= (uint32_t)c.T) return;
-  const Raw<E, V> mine = pm_load<E, V>(src + (size_t)t * c.D.x_stride + (size_t)v * V);
-  float f[V];
-  pm_widen<E, V>(mine, f);
-  for (uint32_t k = 0; k < K; k++) {
-    const uint32_t pos = rows_pos(c, c.pl.pos[t * K + k]);
-    if (pos == PM_ROWS_NONE) continue;
-    Raw<E, V> o = mine;
-    if (w) {
-      const float wk = w[t * K + k];
-      float g[V];
-#pragma unroll
-      for (int j = 0; j < V; j++) g[j] = __fmul_rn(f[j], wk);
-      o = pm_narrow<E, V>(g);
-    }
-    pm_store<E, V>(out + (size_t)pos * c.D.rows_stride + (size_t)v * V, o);
-  }
+// A token's threads walk its row and its K rows together, vector by vector, the K accesses of a step in flight at once: the
+// positions and weights are read once a token, and the K dot products stay in a thread's registers until the end.
+//   SPREAD   out[pos] = w src[t]                         otherwise   out[t] = add[t] + sum_k w rows[pos]
+//   DOT      dw[t][k] = <rows[pos], src[t]>
+// G: a power of two, 256 at most (a CTA); grid.y cuts the rows of a few tokens without DOT further. Behind the tokens' CTAs
+// (SPREAD), one an expert for the padding of its group. KB: K rounded up to one of five (10 pairs in a kernel for 16: 147 us instead of 126
+// for 8192 x 2048 bf16 with dot products). Rows that do not start on 16 bytes go value by value, two
+// values of a row a step and 32 warps an SM (8000 x 1001 f16 with dot products, 5 pairs: 74 us; one value a step 81, four values and 8 warps
+// 112), at about half of the speed of 16-byte words.
+// CTAs that an SM is to hold: registers against reads in flight. Rows read as 16-byte words: 2 (8192 x 2048 bf16 with dot products 101 us; 1:
+// 130, 3: 104). Value by value: 4, of many pairs 2 (10 pairs: 4 spilled, 538 us against 363). Rows that are only written: any.
+__host__ __device__ constexpr int rows_ctas(int V, int KB, bool SPREAD, bool DOT) {
+  return SPREAD && !DOT ? 1 : V == 1 && KB <= 8 ? 4 : 2;
 }
-
-// KB: pairs whose reads are in flight together
-template <typename E, int V, int KB>
-__global__ void __launch_bounds__(256) k_rows_gather(RowsCall c, const float *__restrict__ w, const E *__restrict__ rows, const E *add, E *out) {
+template <typename E, int V, int KB, bool SPREAD, bool DOT>
+__global__ void __launch_bounds__(256, rows_ctas(V, KB, SPREAD, DOT)) k_rows(RowsCall c, uint32_t token_ctas, int G, const float *__restrict__ w, const E *__restrict__ src,
+                                              const E *__restrict__ rows, const E *add, E *out, float *__restrict__ dw) {
   pm_pdl();
-  const uint32_t dv = (uint32_t)c.D.d / V, K = c.D.top_k;
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x, t = i / dv, v = i - t * dv;
-  if (t >= (uint32_t)c.T) return;
-  float acc[V] = {};
-  if (add) pm_widen<E, V>(pm_load<E, V>(add + (size_t)t * c.D.x_stride + (size_t)v * V), acc);
-  for (uint32_t k0 = 0; k0 < K; k0 += KB) {
-    Raw<E, V> r[KB];
-    float wk[KB];
-    bool has[KB];
-#pragma unroll
-    for (int k = 0; k < KB; k++) {
-      const uint32_t pos = k0 + k < K ? rows_pos(c, c.pl.pos[t * K + k0 + k]) : PM_ROWS_NONE;
-      has[k] = pos != PM_ROWS_NONE;
-      if (has[k]) {
-        r[k] = pm_load<E, V>(rows + (size_t)pos * c.D.rows_stride + (size_t)v * V);
-        wk[k] = w ? w[t * K + k0 + k] : 1.0f;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < KB; k++)
-      if (has[k]) {
-        float f[V];
-        pm_widen<E, V>(r[k], f);
-#pragma unroll
-        for (int j = 0; j < V; j++) acc[j] = __fmaf_rn(wk[k], f[j], acc[j]);
-      }
-  }
-  pm_store<E, V>(out + (size_t)t * c.D.x_stride + (size_t)v * V, pm_narrow<E, V>(acc));
-}
-
-// ---------------------------------------------------------------------------
-// gradients with the weights' dot products: W warps a token
-// ---------------------------------------------------------------------------
-// A lane walks its vectors of the token's row and of its K rows, so the K dot products stay in its registers; lanes are
-// summed once a token. SPREAD: rows read, out[pos] = w src[t] written (the gradient of collect). Otherwise out[t] = sum of
-// w rows[pos] (the gradient of dispatch). Behind the tokens' CTAs (SPREAD), one an expert for the padding.
-template <typename E, int V, int KB, bool SPREAD>
-__global__ void __launch_bounds__(256) k_rows_dot(RowsCall c, uint32_t token_ctas, int W, const float *__restrict__ w, const E *__restrict__ src,
-                                                  const E *__restrict__ rows, E *__restrict__ out, float *__restrict__ dw) {
-  pm_pdl();
-  __shared__ float sums[8][KB];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ float sums[DOT ? 8 : 1][KB];
+  const int tid = threadIdx.x;
   const uint32_t dv = (uint32_t)c.D.d / V, K = c.D.top_k;
   if (SPREAD && blockIdx.x >= token_ctas) {
     const uint32_t e = blockIdx.x - token_ctas;
+    if (blockIdx.y) return;
     const uint32_t from = c.pl.offset[e] + c.pl.count[e], to = c.pl.offset[e + 1];
     rows_zero<E, V>(c, out, from, (uint32_t)min((int64_t)to, c.pl.max_rows));
     return;
   }
-  const uint32_t t = blockIdx.x * (8 / W) + warp / W;
-  const int part = warp % W;
+  const uint32_t t = blockIdx.x * (256 / G) + tid / G;
+  const bool live = t < (uint32_t)c.T;
+  const uint32_t first = blockIdx.y * G + tid % G, step = gridDim.y * G;
   uint32_t pos[KB];
-  float wk[KB], dot[KB];
+  float wk[KB];
+  DotOf<V> dot[KB];
 #pragma unroll
   for (int k = 0; k < KB; k++) {
-    const bool in = t < (uint32_t)c.T && k < (int)K;
-    pos[k] = in ? rows_pos(c, c.pl.pos[t * K + k]) : PM_ROWS_NONE;
+    const bool in = live && k < (int)K;
+    pos[k] = in ? c.pl.pos[t * K + k] : PM_ROWS_NONE;
     wk[k] = in && w ? w[t * K + k] : 1.0f;
-    dot[k] = 0.0f;
+    dot[k] = 0;
   }
-  if (t < (uint32_t)c.T)
-    for (uint32_t v = part * 32 + lane; v < dv; v += 32 * W) {
-      const Raw<E, V> s = pm_load<E, V>(src + (size_t)t * c.D.x_stride + (size_t)v * V);
-      Raw<E, V> r[KB];
 #pragma unroll
-      for (int k = 0; k < KB; k++)
-        if (pos[k] != PM_ROWS_NONE) r[k] = pm_load<E, V>(rows + (size_t)pos[k] * c.D.rows_stride + (size_t)v * V);
-      float f[V], acc[V] = {};
-      pm_widen<E, V>(s, f);
+  for (int k = 0; k < KB; k++) pos[k] = rows_pos(c, pos[k]);
+  // vectors of a step: single values come two at a time, so that their reads are in flight together
+  constexpr int J = V > 1 ? 1 : 2;
+  if (live)
+    for (uint32_t v0 = first; v0 < dv; v0 += step * J) {
+      const size_t row = (size_t)t * c.D.x_stride;
+      Raw<E, V> s[J], r[KB][J];
 #pragma unroll
-      for (int k = 0; k < KB; k++)
-        if (pos[k] != PM_ROWS_NONE) {
-          float g[V], o[V];
-          pm_widen<E, V>(r[k], g);
+      for (int j = 0; j < J; j++) {
+        const uint32_t v = v0 + j * step;
+        if (J > 1 && v >= dv) break;
+        if (SPREAD || DOT) s[j] = pm_load<E, V>(src + row + (size_t)v * V);
+        else if (add) s[j] = pm_load<E, V>(add + row + (size_t)v * V);
+        if (!SPREAD || DOT) {
 #pragma unroll
-          for (int j = 0; j < V; j++) {
-            dot[k] = __fmaf_rn(f[j], g[j], dot[k]);
-            if (SPREAD) o[j] = __fmul_rn(wk[k], f[j]);
-            else acc[j] = __fmaf_rn(wk[k], g[j], acc[j]);
+          for (int k = 0; k < KB; k++) {  // (a pair without a row: zeros, which add nothing)
+            r[k][j] = vf_narrow<E, V>(vf_zero<V>());
+            if (pos[k] != PM_ROWS_NONE) r[k][j] = pm_load<E, V>(rows + (size_t)pos[k] * c.D.rows_stride + (size_t)v * V);
           }
-          if (SPREAD) pm_store<E, V>(out + (size_t)pos[k] * c.D.rows_stride + (size_t)v * V, pm_narrow<E, V>(o));
         }
-      if (!SPREAD) pm_store<E, V>(out + (size_t)t * c.D.x_stride + (size_t)v * V, pm_narrow<E, V>(acc));
+      }
+#pragma unroll
+      for (int j = 0; j < J; j++) {
+        const uint32_t v = v0 + j * step;
+        if (J > 1 && v >= dv) break;
+        const VecF<V> f = (SPREAD || DOT || add) ? vf_widen<E, V>(s[j]) : vf_zero<V>();
+        VecF<V> acc = DOT ? vf_zero<V>() : f;
+#pragma unroll
+        for (int k = 0; k < KB; k++) {
+          if (V == 1 && k >= (int)K) break;
+          if (!SPREAD || DOT) {
+            const VecF<V> g = vf_widen<E, V>(r[k][j]);
+            if (DOT) vf_dot<V>(dot[k], g, f);
+            if (!SPREAD) vf_fma<V>(acc, g, wk[k]);
+          }
+          if (SPREAD && pos[k] != PM_ROWS_NONE)
+            pm_store<E, V>(out + (size_t)pos[k] * c.D.rows_stride + (size_t)v * V, w ? vf_narrow<E, V>(vf_mul<V>(f, wk[k])) : s[j]);
+        }
+        if (!SPREAD) pm_store<E, V>(out + row + (size_t)v * V, vf_narrow<E, V>(acc));
+      }
     }
+  if constexpr (DOT) {
+    const int lanes = G < 32 ? G : 32;
 #pragma unroll
-  for (int k = 0; k < KB; k++) dot[k] = pm_warp_sum_16_1(dot[k]);
-  if (lane == 0) {
-#pragma unroll
-    for (int k = 0; k < KB; k++) sums[warp][k] = dot[k];
-  }
-  __syncthreads();
-  if (part == 0 && lane < (int)K && t < (uint32_t)c.T) {
-    float s = 0.0f;
-    for (int i = 0; i < W; i++) s = __fadd_rn(s, sums[warp + i][lane]);
-    dw[t * K + lane] = s;
+    for (int k = 0; k < KB; k++) {
+      float a = vf_sum(dot[k]);
+      for (int o = lanes / 2; o >= 1; o >>= 1) a = __fadd_rn(a, __shfl_xor_sync(PM_FULL, a, o));
+      if (G <= 32) {
+        if (live && tid % G == 0 && k < (int)K) dw[t * K + k] = a;
+      } else if ((tid & 31) == 0) {
+        sums[tid >> 5][k] = a;
+      }
+    }
+    if (G <= 32) return;
+    __syncthreads();
+    const int in = tid % G;
+    if (live && in < (int)K) {
+      float a = 0.0f;
+      for (int i = 0; i < G / 32; i++) a = __fadd_rn(a, sums[tid / G * (G / 32) + i][in]);
+      dw[t * K + in] = a;
+    }
   }
 }
 
@@ -388,13 +381,33 @@ __global__ void __launch_bounds__(256) k_rows_dot(RowsCall c, uint32_t token_cta
   } while (0)
 
 static uint32_t rows_vectors(const RowsCall &c) { return c.vec ? (uint32_t)c.D.d / (c.D.dtype == PM_TYPE_F32 ? 4 : 8) : (uint32_t)c.D.d; }
-static uint32_t rows_pad_ctas(const RowsCall &c) { return c.D.align > 1 ? (uint32_t)c.D.n_local : 0; }
 
-template <typename E, int V>
-static cudaError_t spread(const Launch &L, const RowsCall &c, const float *w, const void *src, void *out) {
-  const uint32_t ctas = (uint32_t)(((size_t)c.T * rows_vectors(c) + 255) / 256);
-  if (ctas + rows_pad_ctas(c) == 0) return cudaSuccess;
-  return pm_launch(L, k_rows_spread<E, V>, ctas + rows_pad_ctas(c), 256, 0, c, ctas, w, (const E *)src, (E *)out);
+// The threads of a token: as many as its row has vectors, but no more than give every SM 32 warps (4096 x 2048 bf16 back to
+// their tokens: 28 us; 8 warps 31, all 30; with dot products, 8192 tokens: 101, 101, 145). Rows that are only written have one
+// read in flight a thread, so they take all (prompt of 4096 x 7168: 101 us, 112 with 32 warps). Where even CTAs of 256
+// threads leave SMs without work, a row without dot products is cut (grid.y).
+template <typename E, int V, int KB, bool SPREAD, bool DOT>
+static cudaError_t rows_go(const Launch &L, const RowsCall &c, const float *w, const void *src, const void *rows, const void *add, void *out,
+                           float *dw) {
+  const uint32_t dv = rows_vectors(c), pad = SPREAD && c.D.align > 1 ? (uint32_t)c.D.n_local : 0;
+  int G = 4;
+  while (G < 256 && (uint32_t)G < dv && (G < 32 || (SPREAD && !DOT) || (int64_t)c.T * G < (int64_t)32 * 32 * L.n_sm)) G *= 2;
+  const uint32_t ctas = ((uint32_t)c.T * G + 255) / 256;
+  uint32_t cuts = 1;
+  if (!DOT)
+    while (ctas * cuts < 2u * L.n_sm && cuts * G < dv) cuts *= 2;
+  if (ctas + pad == 0) return cudaSuccess;
+  return pm_launch(L, k_rows<E, V, KB, SPREAD, DOT>, dim3(ctas + pad, cuts), 256, 0, c, ctas, G, w, (const E *)src, (const E *)rows, (const E *)add,
+                   (E *)out, dw);
+}
+template <typename E, int V, bool SPREAD, bool DOT>
+static cudaError_t rows_k(const Launch &L, const RowsCall &c, const float *w, const void *src, const void *rows, const void *add, void *out,
+                          float *dw) {
+  if (c.D.top_k <= 4) return rows_go<E, V, 4, SPREAD, DOT>(L, c, w, src, rows, add, out, dw);
+  if (c.D.top_k <= 6) return rows_go<E, V, 6, SPREAD, DOT>(L, c, w, src, rows, add, out, dw);
+  if (c.D.top_k <= 8) return rows_go<E, V, 8, SPREAD, DOT>(L, c, w, src, rows, add, out, dw);
+  if (c.D.top_k <= 12) return rows_go<E, V, 12, SPREAD, DOT>(L, c, w, src, rows, add, out, dw);
+  return rows_go<E, V, 16, SPREAD, DOT>(L, c, w, src, rows, add, out, dw);
 }
 
 template <typename E, int V>
@@ -410,56 +423,22 @@ cudaError_t launch_rows_dispatch(const Launch &L, const RowsCall &c, const uint3
     ROWS_TYPES(CALL);
 #undef CALL
   }
-  const cudaError_t e = pm_launch(L, k_rows_sort, SORT_CTAS, SORT_WARPS * 32, 0, c, ids, w);
+  const uint32_t P = (uint32_t)c.T * c.D.top_k, steps = (P + SORT_RUN * SORT_CLUSTERS - 1) / (SORT_RUN * SORT_CLUSTERS);
+  const uint32_t clusters = (P + SORT_RUN * steps - 1) / (SORT_RUN * steps);
+  const cudaError_t e = pm_launch(L, k_rows_sort, clusters * SORT_CTAS, SORT_THREADS, 0, c, steps, ids, w);
   if (e != cudaSuccess || !x) return e;
-#define CALL(E, V) spread<E, V>(L, c, scale ? w : nullptr, x, rows)
-  ROWS_TYPES(CALL);
-#undef CALL
-}
-
-template <typename E, int V, int KB, bool SPREAD>
-static cudaError_t dot(const Launch &L, const RowsCall &c, const float *w, const void *src, const void *rows, void *out, float *dw) {
-  // warps a token: as many as give every SM 16 warps, while each has a vector a lane
-  int W = 1;
-  while (W < 8 && (int64_t)c.T * W < 16 * L.n_sm && rows_vectors(c) > (uint32_t)(32 * W)) W *= 2;
-  const uint32_t ctas = ((uint32_t)c.T * W + 7) / 8, pad = SPREAD ? rows_pad_ctas(c) : 0;
-  if (ctas + pad == 0) return cudaSuccess;
-  return pm_launch(L, k_rows_dot<E, V, KB, SPREAD>, ctas + pad, 256, 0, c, ctas, W, w, (const E *)src, (const E *)rows, (E *)out, dw);
-}
-template <typename E, int V, bool SPREAD>
-static cudaError_t dot_k(const Launch &L, const RowsCall &c, const float *w, const void *src, const void *rows, void *out, float *dw) {
-  if (c.D.top_k <= 4) return dot<E, V, 4, SPREAD>(L, c, w, src, rows, out, dw);
-  if (c.D.top_k <= 8) return dot<E, V, 8, SPREAD>(L, c, w, src, rows, out, dw);
-  return dot<E, V, 16, SPREAD>(L, c, w, src, rows, out, dw);
-}
-
-template <typename E, int V>
-static cudaError_t gather(const Launch &L, const RowsCall &c, const float *w, const void *rows, const void *add, void *out) {
-  const uint32_t ctas = (uint32_t)(((size_t)c.T * rows_vectors(c) + 255) / 256);
-  if (ctas == 0) return cudaSuccess;
-  if (c.D.top_k <= 4) return pm_launch(L, k_rows_gather<E, V, 4>, ctas, 256, 0, c, w, (const E *)rows, (const E *)add, (E *)out);
-  return pm_launch(L, k_rows_gather<E, V, 8>, ctas, 256, 0, c, w, (const E *)rows, (const E *)add, (E *)out);
+  return launch_rows_spread(L, c, scale ? w : nullptr, x, nullptr, rows, nullptr);
 }
 
 cudaError_t launch_rows_gather(const Launch &L, const RowsCall &c, const float *w, const void *rows, const void *add, const void *x, void *out,
                                float *dw) {
-  if (dw) {
-#define CALL(E, V) dot_k<E, V, false>(L, c, w, x, rows, out, dw)
-    ROWS_TYPES(CALL);
-#undef CALL
-  }
-#define CALL(E, V) gather<E, V>(L, c, w, rows, add, out)
+#define CALL(E, V) (dw ? rows_k<E, V, false, true>(L, c, w, x, rows, nullptr, out, dw) : rows_k<E, V, false, false>(L, c, w, nullptr, rows, add, out, nullptr))
   ROWS_TYPES(CALL);
 #undef CALL
 }
 
 cudaError_t launch_rows_spread(const Launch &L, const RowsCall &c, const float *w, const void *src, const void *rows, void *out, float *dw) {
-  if (dw) {
-#define CALL(E, V) dot_k<E, V, true>(L, c, w, src, rows, out, dw)
-    ROWS_TYPES(CALL);
-#undef CALL
-  }
-#define CALL(E, V) spread<E, V>(L, c, w, src, out)
+#define CALL(E, V) (dw ? rows_k<E, V, true, true>(L, c, w, src, rows, nullptr, out, dw) : rows_k<E, V, true, false>(L, c, w, src, nullptr, nullptr, out, nullptr))
   ROWS_TYPES(CALL);
 #undef CALL
 }

@@ -117,3 +117,72 @@ __device__ __forceinline__ float dot8(const F8 &a, const F8 &b) {
   pm_unpack2(s, x, y);
   return __fadd_rn(x, y);
 }
+
+// V f32 values, in pairs where there are any
+template <int V> struct VecF {
+  uint64_t p[V / 2];
+};
+template <> struct VecF<1> {
+  float p[1];
+};
+template <typename E, int V> __device__ __forceinline__ VecF<V> vf_widen(const Raw<E, V> &r) {
+  VecF<V> f;
+  if constexpr (V == 1) f.p[0] = pm_to_f32(r.v[0]);
+  else {
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) f.p[i] = pm_widen2(&r.v[2 * i]);
+  }
+  return f;
+}
+template <typename E, int V> __device__ __forceinline__ Raw<E, V> vf_narrow(const VecF<V> &f) {
+  Raw<E, V> r;
+  if constexpr (V == 1) r.v[0] = pm_from_f32<E>(f.p[0]);
+  else {
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) {
+      float a, b;
+      pm_unpack2(f.p[i], a, b);
+      pm_narrow2(&r.v[2 * i], a, b);
+    }
+  }
+  return r;
+}
+template <int V> __device__ __forceinline__ VecF<V> vf_zero() {
+  VecF<V> f;
+#pragma unroll
+  for (int i = 0; i < (V == 1 ? 1 : V / 2); i++) f.p[i] = 0;
+  return f;
+}
+template <int V> __device__ __forceinline__ VecF<V> vf_mul(const VecF<V> &a, float s) {
+  VecF<V> f;
+  if constexpr (V == 1) f.p[0] = __fmul_rn(a.p[0], s);
+  else {
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) f.p[i] = pm_mul2(a.p[i], pm_pack2(s, s));
+  }
+  return f;
+}
+template <int V> __device__ __forceinline__ void vf_fma(VecF<V> &acc, const VecF<V> &a, float s) {
+  if constexpr (V == 1) acc.p[0] = __fmaf_rn(a.p[0], s, acc.p[0]);
+  else {
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) acc.p[i] = pm_fma2(a.p[i], pm_pack2(s, s), acc.p[i]);
+  }
+}
+// running sums of a b: two, or one where V is one
+template <int V> struct DotT { using T = uint64_t; };
+template <> struct DotT<1> { using T = float; };
+template <int V> using DotOf = typename DotT<V>::T;
+template <int V> __device__ __forceinline__ void vf_dot(DotOf<V> &acc, const VecF<V> &a, const VecF<V> &b) {
+  if constexpr (V == 1) acc = __fmaf_rn(a.p[0], b.p[0], acc);
+  else {
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) acc = pm_fma2(a.p[i], b.p[i], acc);
+  }
+}
+__device__ __forceinline__ float vf_sum(float v) { return v; }
+__device__ __forceinline__ float vf_sum(uint64_t v) {
+  float a, b;
+  pm_unpack2(v, a, b);
+  return __fadd_rn(a, b);
+}
