@@ -16,13 +16,12 @@
 
 namespace cg = cooperative_groups;
 
-// A thread holds 8 values of a row; a row's group has tpr threads (whole warps) in each of cl CTAs (a cluster, for rows of
-// more than 8,192 values), a CTA has rpb groups, each with rows of its own. Rows of a group follow one another; a thread
-// copies its own values of the next ones into its own slots of shared memory (cp.async) while it works on one, so that the bytes
-// in flight do not depend on registers and no thread waits for another's copy.
-#define NORM_VALUES 8
-#define NORM_GRAD_THREADS 896  // ... backward: 72
-#define NORM_THREADS 1024      // threads resident on an SM, forward: 64 registers each
+// A thread holds N values of a row; a row's group has tpr threads (whole warps) in each of cl CTAs (a cluster, for rows that
+// the registers of an SM do not hold), a CTA has rpb groups, each with rows of its own. Rows of a group follow one another; a
+// thread copies its own values of the next ones into its own slots of shared memory (cp.async) while it works on one, so that
+// the bytes in flight do not depend on registers and no thread waits for another's copy.
+#define NORM_FWD_VALUES 8192   // values of rows resident on an SM
+#define NORM_GRAD_VALUES(n) ((n) == 16 ? 8192 : 7168)  // ... backward, with n values a thread: 512 threads of 128 registers, 896 of 72
 #define NORM_SMEM 233472      // bytes of shared memory of an SM, of which every CTA takes
 #define NORM_SMEM_CTA 2560    // ... these for its sums and for itself
 struct NormShape {
@@ -32,14 +31,14 @@ struct NormShape {
   int per_sm;         // CTAs resident on an SM
   int threads() const { return tpr * rpb; }
 };
-static NormShape norm_shape(int d, int sm_threads) {
+static NormShape norm_shape(int d, int n, int sm_values) {
   NormShape s = {};
-  const int need = (d + NORM_VALUES - 1) / NORM_VALUES;
+  const int need = (d + n - 1) / n, most = sm_values / n;
   s.cl = 1;
-  while ((need + s.cl - 1) / s.cl > sm_threads) s.cl *= 2;
+  while ((need + s.cl - 1) / s.cl > most) s.cl *= 2;
   s.tpr = ((need + s.cl - 1) / s.cl + 31) / 32 * 32;
   s.rpb = s.cl == 1 && s.tpr < 256 ? 256 / s.tpr : 1;
-  s.per_sm = sm_threads / s.threads();
+  s.per_sm = most / s.threads();
   return s;
 }
 
@@ -108,8 +107,8 @@ __device__ __forceinline__ float norm_inv(float sum, float inv_d, float eps) {
 }
 
 // the thread's 8 values of a row as vectors of V: vector j is columns col0 + j * step ...
-template <typename E, int V> struct NormRow {
-  static constexpr int J = NORM_VALUES / V;
+template <typename E, int V, int N> struct NormRow {
+  static constexpr int J = N / V;
   Raw<E, V> v[J];
   __device__ __forceinline__ void load(const void *base, size_t at, const NormPlace &p, int d) {
 #pragma unroll
@@ -122,19 +121,19 @@ template <typename E, int V> struct NormRow {
       }
     }
   }
-  __device__ __forceinline__ F8 widen() const {
-    F8 f;
+  __device__ __forceinline__ VecF<N> widen() const {
+    VecF<N> f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < N / 2; i++) {
       if constexpr (V == 1) f.p[i] = pm_pack2(pm_to_f32(v[2 * i].v[0]), pm_to_f32(v[2 * i + 1].v[0]));
       else f.p[i] = pm_widen2(&v[2 * i / V].v[2 * i % V]);
     }
     return f;
   }
-  __device__ __forceinline__ static void store(void *base, size_t at, const NormPlace &p, int d, const F8 &f) {
-    float g[NORM_VALUES];
+  __device__ __forceinline__ static void store(void *base, size_t at, const NormPlace &p, int d, const VecF<N> &f) {
+    float g[N];
 #pragma unroll
-    for (int i = 0; i < 4; i++) pm_unpack2(f.p[i], g[2 * i], g[2 * i + 1]);
+    for (int i = 0; i < N / 2; i++) pm_unpack2(f.p[i], g[2 * i], g[2 * i + 1]);
 #pragma unroll
     for (int j = 0; j < J; j++) {
       const int col = p.col0 + j * p.tpr * p.cl * V;
@@ -146,12 +145,12 @@ template <typename E, int V> struct NormRow {
   }
 };
 // weights of the thread's columns, offset added; ones where there are none
-template <typename W, int V>
-__device__ __forceinline__ F8 norm_weights(const void *w, float offset, const NormPlace &p, int d) {
-  if (!w) return F8::all(1.0f);
-  NormRow<W, V> r;
+template <typename W, int V, int N>
+__device__ __forceinline__ VecF<N> norm_weights(const void *w, float offset, const NormPlace &p, int d) {
+  if (!w) return vf_all<N>(1.0f);
+  NormRow<W, V, N> r;
   r.load(w, 0, p, d);
-  return r.widen() + F8::all(offset);
+  return r.widen() + vf_all<N>(offset);
 }
 
 // The thread's slots of shared memory: 16 bytes each, `pitch` bytes (all threads' of the CTA) apart. Addresses of the shared
@@ -167,21 +166,22 @@ struct NormSlots {
   __device__ __forceinline__ static void put(uint32_t a, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
   }
-  __device__ __forceinline__ void put8(int i, const F8 &f) const {
-    asm volatile("st.shared.v2.u64 [%0], {%1, %2};" ::"r"(at(i)), "l"(f.p[0]), "l"(f.p[1]) : "memory");
-    asm volatile("st.shared.v2.u64 [%0], {%1, %2};" ::"r"(at(i + 1)), "l"(f.p[2]), "l"(f.p[3]) : "memory");
+  template <int N> __device__ __forceinline__ void put_vec(int i, const VecF<N> &f) const {
+#pragma unroll
+    for (int j = 0; j < N / 4; j++)
+      asm volatile("st.shared.v2.u64 [%0], {%1, %2};" ::"r"(at(i + j)), "l"(f.p[2 * j]), "l"(f.p[2 * j + 1]) : "memory");
   }
-  __device__ __forceinline__ F8 get8(int i) const {
-    F8 f;
-    asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(f.p[0]), "=l"(f.p[1]) : "r"(at(i)));
-    asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(f.p[2]), "=l"(f.p[3]) : "r"(at(i + 1)));
+  template <int N> __device__ __forceinline__ VecF<N> get_vec(int i) const {
+    VecF<N> f;
+#pragma unroll
+    for (int j = 0; j < N / 4; j++) asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(f.p[2 * j]), "=l"(f.p[2 * j + 1]) : "r"(at(i + j)));
     return f;
   }
 };
 __device__ __forceinline__ NormSlots norm_slots(uint4 *all) { return {(uint32_t)__cvta_generic_to_shared(all + threadIdx.x), blockDim.x * 16}; }
 // The streams of a group's rows: with RING, stream k of a stage is slot k * J behind the stage's `row`; without, a load.
-template <typename E, int V, bool RING> struct NormRing {
-  static constexpr int J = NORM_VALUES / V;
+template <typename E, int V, int N, bool RING> struct NormRing {
+  static constexpr int J = N / V;
   NormSlots slots;
   int first, streams, stages;
   // (columns behind the row are never copied: they stay zero)
@@ -210,7 +210,7 @@ template <typename E, int V, bool RING> struct NormRing {
       else asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
   }
-  __device__ __forceinline__ void get(NormRow<E, V> &r, uint32_t row, int k, const void *base, size_t at, const NormPlace &p, int d) const {
+  __device__ __forceinline__ void get(NormRow<E, V, N> &r, uint32_t row, int k, const void *base, size_t at, const NormPlace &p, int d) const {
     if constexpr (RING) {
 #pragma unroll
       for (int j = 0; j < J; j++) *(uint4 *)&r.v[j] = NormSlots::get(row + (k * J + j) * slots.pitch);
@@ -246,8 +246,8 @@ template <typename W> __device__ __forceinline__ float norm_token_gate(const Nor
 //   NORM_BEFORE    the norm before the next block only, every stream
 enum NormMode { NORM_ANY, NORM_SANDWICH, NORM_BEFORE };
 
-template <typename E, typename W, int V, bool CLUSTER, bool RING, NormMode MODE>
-__global__ void __launch_bounds__(NORM_THREADS) k_block_norm(NormCall c, int tpr, int rpb, int cl, int stages) {
+template <typename E, typename W, int V, int N, bool CLUSTER, bool RING, NormMode MODE>
+__global__ void __launch_bounds__(NORM_FWD_VALUES / N) k_block_norm(NormCall c, int tpr, int rpb, int cl, int stages) {
   pm_pdl();
   extern __shared__ uint4 slots[];
   __shared__ NormRed<1> red;
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_block_norm(NormCall c, int tpr
   const bool post = ANY ? c.D.flags & PM_NORM_POST : MODE == NORM_SANDWICH, pre = ANY ? c.D.flags & PM_NORM_PRE : true;
   const bool has_x = ANY ? c.x != nullptr : true, has_f = ANY ? c.f != nullptr : true, has_r = ANY ? c.r != nullptr : true;
   const int i_x = has_f ? 1 : 0;
-  const NormRing<E, V, RING> ring = {norm_slots(slots), 0, i_x + (has_x ? 1 : 0), stages};
+  const NormRing<E, V, N, RING> ring = {norm_slots(slots), 0, i_x + (has_x ? 1 : 0), stages};
   const int t0 = (int)(blockIdx.x / at.cl) * rpb + at.group;
   auto copy = [&](int stage, int t) {
     if (t < c.T) {
@@ -271,12 +271,12 @@ __global__ void __launch_bounds__(NORM_THREADS) k_block_norm(NormCall c, int tpr
   ring.clear();
   if constexpr (RING)
     for (int s = 0; s < stages; s++) copy(s, t0 + s * groups);
-  F8 wp = norm_weights<W, V>(post ? c.w_post : nullptr, c.D.offset_post, at, d);  // gate and post weight
-  const F8 wn = norm_weights<W, V>(pre ? c.w_pre : nullptr, c.D.offset_pre, at, d);
-  if (c.D.gate == PM_NORM_GATE_CHANNEL) wp = wp * norm_weights<W, V>(c.gate, 0.0f, at, d);
+  VecF<N> wp = norm_weights<W, V, N>(post ? c.w_post : nullptr, c.D.offset_post, at, d);  // gate and post weight
+  const VecF<N> wn = norm_weights<W, V, N>(pre ? c.w_pre : nullptr, c.D.offset_pre, at, d);
+  if (c.D.gate == PM_NORM_GATE_CHANNEL) wp = wp * norm_weights<W, V, N>(c.gate, 0.0f, at, d);
   int turn = 0, stage = 0;
   for (int t = t0; t < c.T; t += groups) {
-    NormRow<E, V> xr, fr;
+    NormRow<E, V, N> xr, fr;
     ring.wait();
     const uint32_t row = ring.row(stage);
     if (has_f) ring.get(fr, row, 0, c.f, norm_row(t, c.D.f_stride), at, d);
@@ -285,22 +285,22 @@ __global__ void __launch_bounds__(NORM_THREADS) k_block_norm(NormCall c, int tpr
       copy(stage, t + stages * groups);
       stage = stage + 1 == stages ? 0 : stage + 1;
     }
-    F8 r = has_x ? xr.widen() * c.D.alpha : F8::all(0.0f);
+    VecF<N> r = has_x ? xr.widen() * c.D.alpha : vf_all<N>(0.0f);
     if (has_f) {
-      const F8 f = fr.widen();
+      const VecF<N> f = fr.widen();
       float s = __fmul_rn(c.D.beta, norm_token_gate<W>(c, t));
       if (post) {
-        float sum[1] = {dot8(f, f)};
+        float sum[1] = {vf_dot(f, f)};
         norm_sum<1, CLUSTER>(sum, at, red, peer, turn);
         s = __fmul_rn(s, norm_inv(sum[0], c.inv_d, c.D.eps_post));
       }
-      r = fma8(f * wp, s, r);
+      r = vf_fma(f * wp, s, r);
     }
-    if (has_r) NormRow<E, V>::store(c.r, norm_row(t, c.D.r_stride), at, d, r);
+    if (has_r) NormRow<E, V, N>::store(c.r, norm_row(t, c.D.r_stride), at, d, r);
     if (pre) {
-      float sum[1] = {dot8(r, r)};
+      float sum[1] = {vf_dot(r, r)};
       norm_sum<1, CLUSTER>(sum, at, red, peer, turn);
-      NormRow<E, V>::store(c.n, norm_row(t, c.D.n_stride), at, d, r * wn * norm_inv(sum[0], c.inv_d, c.D.eps_pre));
+      NormRow<E, V, N>::store(c.n, norm_row(t, c.D.n_stride), at, d, r * wn * norm_inv(sum[0], c.inv_d, c.D.eps_pre));
     }
   }
   if constexpr (CLUSTER) cg::this_cluster().sync();  // no CTA leaves while another may still write its sums here
@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(NORM_THREADS) k_block_norm(NormCall c, int tpr
 // are read again from the ring each time and the weights lie beside it (f32, the thread's own columns): the 16 sums of the
 // weights' gradients fill the registers. A CTA adds up its groups and leaves a row of sums in parts[kind][CTA][d], which
 // k_norm_sum_parts adds up. No atomics.
-template <typename E, typename W, int V, bool CLUSTER, bool RING, NormMode MODE>
-__global__ void __launch_bounds__(NORM_GRAD_THREADS) k_block_norm_grad(NormCall c, int tpr, int rpb, int cl, int stages) {
+template <typename E, typename W, int V, int N, bool CLUSTER, bool RING, NormMode MODE>
+__global__ void __launch_bounds__(NORM_GRAD_VALUES(N) / N) k_block_norm_grad(NormCall c, int tpr, int rpb, int cl, int stages) {
   pm_pdl();
   extern __shared__ uint4 slots[];
   __shared__ NormRed<3> red3;
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(NORM_GRAD_THREADS) k_block_norm_grad(NormCall 
   const NormSlots own = norm_slots(slots);
   // slots: the pre weight, post weight times the channel's gate, the ring
   const int i_f = pre ? 2 : 0, i_dr = i_f + (use_f ? 1 : 0);
-  const NormRing<E, V, RING> ring = {own, 4, i_dr + (has_dr ? 1 : 0), stages};
+  const NormRing<E, V, N, RING> ring = {own, N / 2, i_dr + (has_dr ? 1 : 0), stages};
   const int t0 = part * rpb + at.group;
   auto copy = [&](int stage, int t) {
     if (t < c.T) {
@@ -345,30 +345,30 @@ __global__ void __launch_bounds__(NORM_GRAD_THREADS) k_block_norm_grad(NormCall 
   ring.clear();
   if constexpr (RING)
     for (int s = 0; s < stages; s++) copy(s, t0 + s * groups);
-  own.put8(0, norm_weights<W, V>(pre ? c.w_pre : nullptr, c.D.offset_pre, at, d));
-  own.put8(2, norm_weights<W, V>(post ? c.w_post : nullptr, c.D.offset_post, at, d) * norm_weights<W, V>(channel ? c.gate : nullptr, 0.0f, at, d));
-  F8 a_pre = F8::all(0.0f), a_dk = F8::all(0.0f);
+  own.template put_vec<N>(0, norm_weights<W, V, N>(pre ? c.w_pre : nullptr, c.D.offset_pre, at, d));
+  own.template put_vec<N>(N / 4, norm_weights<W, V, N>(post ? c.w_post : nullptr, c.D.offset_post, at, d) * norm_weights<W, V, N>(channel ? c.gate : nullptr, 0.0f, at, d));
+  VecF<N> a_pre = vf_all<N>(0.0f), a_dk = vf_all<N>(0.0f);
   int turn3 = 0, turn = 0, stage = 0;
   for (int t = t0; t < c.T; t += groups) {
     const size_t at_r = norm_row(t, c.D.r_stride), at_f = norm_row(t, c.D.f_stride), at_n = norm_row(t, c.D.n_stride);
     const uint32_t row = ring.row(stage);
-    NormRow<E, V> raw, fr;
+    NormRow<E, V, N> raw, fr;
     float sum[3] = {0.0f, 0.0f, 0.0f};
     ring.wait();
     if (pre) {
       ring.get(raw, row, 0, c.x, at_r, at, d);
-      const F8 r = raw.widen();
+      const VecF<N> r = raw.widen();
       ring.get(raw, row, 1, c.dn, at_n, at, d);
-      sum[0] = dot8(r, r);
-      sum[1] = dot8(raw.widen() * own.get8(0), r);
+      sum[0] = vf_dot(r, r);
+      sum[1] = vf_dot(raw.widen() * own.template get_vec<N>(0), r);
     }
     if (use_f) ring.get(fr, row, i_f, c.f, at_f, at, d);
     if (post) {
-      const F8 f = fr.widen();
-      sum[2] = dot8(f, f);
+      const VecF<N> f = fr.widen();
+      sum[2] = vf_dot(f, f);
     }
     if (pre || post) norm_sum<3, CLUSTER>(sum, at, red3, peer3, turn3);
-    F8 D = F8::all(0.0f);
+    VecF<N> D = vf_all<N>(0.0f);
     if (has_dr) {
       ring.get(raw, row, i_dr, c.dr, at_r, at, d);
       D = raw.widen();
@@ -377,29 +377,29 @@ __global__ void __launch_bounds__(NORM_GRAD_THREADS) k_block_norm_grad(NormCall 
       const float s2 = norm_inv(sum[0], c.inv_d, c.D.eps_pre);
       const float m = __fmul_rn(__fmul_rn(s2, s2), __fmul_rn(sum[1], c.inv_d));
       ring.get(raw, row, 0, c.x, at_r, at, d);
-      const F8 r = raw.widen();
+      const VecF<N> r = raw.widen();
       ring.get(raw, row, 1, c.dn, at_n, at, d);
-      const F8 dn = raw.widen();
-      a_pre = fma8(dn, r * s2, a_pre);
-      D = fma8(fma8(r, -m, dn * own.get8(0)), s2, D);
+      const VecF<N> dn = raw.widen();
+      a_pre = vf_fma(dn, r * s2, a_pre);
+      D = vf_fma(vf_fma(r, -m, dn * own.template get_vec<N>(0)), s2, D);
     }
     if constexpr (RING) {  // (f is in registers)
       copy(stage, t + stages * groups);
       stage = stage + 1 == stages ? 0 : stage + 1;
     }
-    if (has_dx) NormRow<E, V>::store(c.dx, norm_row(t, c.D.x_stride), at, d, D * c.D.alpha);
+    if (has_dx) NormRow<E, V, N>::store(c.dx, norm_row(t, c.D.x_stride), at, d, D * c.D.alpha);
     if (!use_f && !has_df) continue;
     // D becomes beta g D, g of the token, then beta g D (o1 + w_post) of either gate; k = f s1
     const float gt = MODE == NORM_BEFORE ? 1.0f : norm_token_gate<W>(c, t);
     float s1 = 1.0f, mean = 0.0f;
     if (use_f) {
       if (post) s1 = norm_inv(sum[2], c.inv_d, c.D.eps_post);
-      const F8 k = fr.widen() * s1;
+      const VecF<N> k = fr.widen() * s1;
       D = D * c.D.beta;
-      if (post || channel) a_dk = fma8(D * gt, k, a_dk);
-      D = D * own.get8(2);
+      if (post || channel) a_dk = vf_fma(D * gt, k, a_dk);
+      D = D * own.template get_vec<N>(N / 4);
       if (post || token) {
-        float dot[1] = {dot8(D, k)};
+        float dot[1] = {vf_dot(D, k)};
         norm_sum<1, CLUSTER>(dot, at, red, peer, turn);
         if (token && c.dgate && at.rank == 0 && at.warp == 0 && at.lane == 0) c.dgate[t] = dot[0];
         mean = __fmul_rn(__fmul_rn(dot[0], gt), c.inv_d);
@@ -409,8 +409,8 @@ __global__ void __launch_bounds__(NORM_GRAD_THREADS) k_block_norm_grad(NormCall 
       D = D * c.D.beta;
     }
     if (has_df) {
-      if (post) D = fma8(fr.widen() * s1, -mean, D) * s1;
-      NormRow<E, V>::store(c.df, at_f, at, d, D);
+      if (post) D = vf_fma(fr.widen() * s1, -mean, D) * s1;
+      NormRow<E, V, N>::store(c.df, at_f, at, d, D);
     }
   }
   // The CTA's groups, kind by kind, columns of a thread as it holds them. With K = sum over t of beta g_t D k, dw_post is K times
@@ -420,41 +420,30 @@ __global__ void __launch_bounds__(NORM_GRAD_THREADS) k_block_norm_grad(NormCall 
   for (int kind = 0; kind < 2; kind++) {
     const bool on = kind == 0 ? pre && c.dw_pre : (post && c.dw_post) || (channel && c.dgate);
     if (!on) continue;
-    F8 sums = kind == 0 ? a_pre : a_dk;
+    VecF<N> sums = kind == 0 ? a_pre : a_dk;
     if (rpb > 1) {
       __syncthreads();
-      own.put8(0, sums);  // (the weights have served)
+      own.template put_vec<N>(0, sums);  // (the weights have served)
       __syncthreads();
       if (at.group == 0)
-        for (int g = 1; g < rpb; g++) sums = sums + NormSlots{own.mine + g * tpr * 16, own.pitch}.get8(0);
+        for (int g = 1; g < rpb; g++) sums = sums + NormSlots{own.mine + g * tpr * 16, own.pitch}.template get_vec<N>(0);
     }
-    auto leave = [&](int which, const F8 &s) {
-      float a[NORM_VALUES];
-#pragma unroll
-      for (int i = 0; i < 4; i++) pm_unpack2(s.p[i], a[2 * i], a[2 * i + 1]);
-      float *to = c.parts + ((size_t)which * n_parts + part) * d;
-#pragma unroll
-      for (int j = 0; j < NORM_VALUES / V; j++) {
-        const int col = at.col0 + j * tpr * at.cl * V;
-#pragma unroll
-        for (int i = 0; i < V; i++)
-          if (col + i < d) to[col + i] = a[j * V + i];
-      }
-    };
+    auto leave = [&](int which, const VecF<N> &s) { NormRow<float, V, N>::store(c.parts, ((size_t)which * n_parts + part) * d, at, d, s); };
     if (at.group) continue;
     if (kind == 0) leave(0, sums);
     else {
-      if (post && c.dw_post) leave(1, channel ? sums * norm_weights<W, V>(c.gate, 0.0f, at, d) : sums);
-      if (channel && c.dgate) leave(2, post ? sums * norm_weights<W, V>(c.w_post, c.D.offset_post, at, d) : sums);
+      if (post && c.dw_post) leave(1, channel ? sums * norm_weights<W, V, N>(c.gate, 0.0f, at, d) : sums);
+      if (channel && c.dgate) leave(2, post ? sums * norm_weights<W, V, N>(c.w_post, c.D.offset_post, at, d) : sums);
     }
   }
   if constexpr (CLUSTER) cg::this_cluster().sync();
 }
 
-// out[kind][col] = sum over the parts, 8 runs of parts a CTA of 32 columns, runs added in order
-__global__ void __launch_bounds__(256) k_norm_sum_parts(const float *__restrict__ parts, int n_parts, int d, float *o0, float *o1, float *o2) {
+// out[kind][col] = sum over the parts: a CTA has 32 columns, a warp the parts 32 apart, warps are added in order (8 warps a CTA:
+// 17 us instead of 14 for the gradient of 4096 x 512)
+__global__ void __launch_bounds__(1024) k_norm_sum_parts(const float *__restrict__ parts, int n_parts, int d, float *o0, float *o1, float *o2) {
   pm_pdl();
-  __shared__ float red[8][32];
+  __shared__ float red[32][32];
   float *out = blockIdx.y == 0 ? o0 : blockIdx.y == 1 ? o1 : o2;
   if (!out) return;
   const int lane = threadIdx.x & 31, run = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
@@ -462,13 +451,13 @@ __global__ void __launch_bounds__(256) k_norm_sum_parts(const float *__restrict_
   float s = 0.0f;
   if (col < d) {
 #pragma unroll 4
-    for (int i = run; i < n_parts; i += 8) s = __fadd_rn(s, p[(size_t)i * d + col]);
+    for (int i = run; i < n_parts; i += 32) s = __fadd_rn(s, p[(size_t)i * d + col]);
   }
   red[run][lane] = s;
   __syncthreads();
   if (run == 0 && col < d) {
 #pragma unroll
-    for (int i = 1; i < 8; i++) s = __fadd_rn(s, red[i][lane]);
+    for (int i = 1; i < 32; i++) s = __fadd_rn(s, red[i][lane]);
     out[col] = s;
   }
 }
@@ -482,7 +471,18 @@ static int norm_parts(const NormShape &s, int T, int n_sm) {
   const int need = (T + s.rpb - 1) / s.rpb;
   return need < most ? need : most;
 }
-size_t norm_parts_floats(const pm_norm_desc &D, int T, int n_sm) { return (size_t)3 * norm_parts(norm_shape(D.d, NORM_GRAD_THREADS), T, n_sm) * D.d; }
+// Values a thread holds where rows are whole 16-byte words. Backward: 16 of the 16-bit types, half the threads for the same sums (4096 x 2048 bf16
+// 31 -> 28 us, x 4096 60 -> 56, x 7168 even), 8 of f32, whose rings are twice the size (4096 x 7168: 145 us, 159 with 16). Forward:
+// 16 for rows of up to 2,048 16-bit values (16384 x 512: 11.6 -> 9.9 us, x 2048 52.4 -> 50.9; 8192 x 4096: 55.5 -> 58.0).
+static int norm_values(const pm_norm_desc &D, bool grad) { return D.dtype != PM_TYPE_F32 && (grad || D.d <= 2048) ? 16 : 8; }
+size_t norm_parts_floats(const pm_norm_desc &D, int T, int n_sm) {
+  size_t most = 0;  // (of both forms of a row: which one is taken goes by the buffers)
+  for (int n : {8, norm_values(D, true)}) {
+    const size_t f = (size_t)3 * norm_parts(norm_shape(D.d, n, NORM_GRAD_VALUES(n)), T, n_sm) * D.d;
+    if (f > most) most = f;
+  }
+  return most;
+}
 
 // the rows of `row` slots that fit into a ring beside `fixed` slots a thread, 3 at most; fewer CTAs on an SM where two would not fit
 static void norm_ring(NormShape &s, int fixed, int row) {
@@ -514,54 +514,64 @@ static cudaError_t norm_launch(const Launch &L, SmemOptIn &opt, void (*kern)(P..
   if (L.count) ++*L.count;
   return cudaLaunchKernelEx(&cfg, kern, c, s.tpr, s.rpb, s.cl, s.stages);
 }
-template <typename E, typename W, int V, bool RING, NormMode MODE, bool GRAD>
+template <typename E, typename W, int V, int N, bool RING, NormMode MODE, bool GRAD>
 static cudaError_t norm_go(const Launch &L, int parts, const NormShape &s, const NormCall &c) {
   static SmemOptIn one, many;
   if constexpr (GRAD)
-    return s.cl > 1 ? norm_launch(L, many, k_block_norm_grad<E, W, V, true, RING, MODE>, parts, s, c)
-                    : norm_launch(L, one, k_block_norm_grad<E, W, V, false, RING, MODE>, parts, s, c);
+    return s.cl > 1 ? norm_launch(L, many, k_block_norm_grad<E, W, V, N, true, RING, MODE>, parts, s, c)
+                    : norm_launch(L, one, k_block_norm_grad<E, W, V, N, false, RING, MODE>, parts, s, c);
   else
-    return s.cl > 1 ? norm_launch(L, many, k_block_norm<E, W, V, true, RING, MODE>, parts, s, c)
-                    : norm_launch(L, one, k_block_norm<E, W, V, false, RING, MODE>, parts, s, c);
+    return s.cl > 1 ? norm_launch(L, many, k_block_norm<E, W, V, N, true, RING, MODE>, parts, s, c)
+                    : norm_launch(L, one, k_block_norm<E, W, V, N, false, RING, MODE>, parts, s, c);
 }
 // the kernels of 16-byte words that go by what the call has
-template <typename E, typename W, int V, bool GRAD>
+template <typename E, typename W, int V, int N, bool GRAD>
 static cudaError_t norm_go_mode(const Launch &L, int parts, const NormShape &s, const NormCall &c) {
   const bool all = GRAD ? c.dr && c.dx && c.df : c.x && c.f && c.r;
   const bool post = c.D.flags & PM_NORM_POST, pre = c.D.flags & PM_NORM_PRE;
-  if (all && pre && post) return norm_go<E, W, V, true, NORM_SANDWICH, GRAD>(L, parts, s, c);
-  if (all && pre && c.D.gate == PM_NORM_GATE_NONE) return norm_go<E, W, V, true, NORM_BEFORE, GRAD>(L, parts, s, c);
-  return norm_go<E, W, V, true, NORM_ANY, GRAD>(L, parts, s, c);
+  if (all && pre && post) return norm_go<E, W, V, N, true, NORM_SANDWICH, GRAD>(L, parts, s, c);
+  if (all && pre && c.D.gate == PM_NORM_GATE_NONE) return norm_go<E, W, V, N, true, NORM_BEFORE, GRAD>(L, parts, s, c);
+  return norm_go<E, W, V, N, true, NORM_ANY, GRAD>(L, parts, s, c);
 }
 
+// rows of 16-byte words, more of them than groups: through rings
+template <typename E, typename W, int V, int N> static cudaError_t norm_forward_ring(const Launch &L, const NormCall &c) {
+  NormShape s = norm_shape(c.D.d, N, NORM_FWD_VALUES);
+  norm_ring(s, 0, ((c.x ? 1 : 0) + (c.f ? 1 : 0)) * N / V);
+  return norm_go_mode<E, W, V, N, false>(L, norm_parts(s, c.T, L.n_sm), s, c);
+}
 template <typename E, typename W, int V> static cudaError_t norm_forward(const Launch &L, const NormCall &c) {
-  NormShape s = norm_shape(c.D.d, NORM_THREADS);
-  // a ring where a group has a second row to fetch
+  const NormShape s = norm_shape(c.D.d, 8, NORM_FWD_VALUES);
+  const int parts = norm_parts(s, c.T, L.n_sm);
   if constexpr (V > 1) {
-    if (c.T > norm_parts(s, c.T, L.n_sm) * s.rpb) {
-      norm_ring(s, 0, ((c.x ? 1 : 0) + (c.f ? 1 : 0)) * NORM_VALUES / V);
-      return norm_go_mode<E, W, V, false>(L, norm_parts(s, c.T, L.n_sm), s, c);
+    if (c.T > parts * s.rpb) {
+      if constexpr (V == 8) if (norm_values(c.D, false) == 16) return norm_forward_ring<E, W, V, 16>(L, c);
+      return norm_forward_ring<E, W, V, 8>(L, c);
     }
   }
-  return norm_go<E, W, V, false, NORM_ANY, false>(L, norm_parts(s, c.T, L.n_sm), s, c);
+  return norm_go<E, W, V, 8, false, NORM_ANY, false>(L, parts, s, c);
+}
+template <typename E, typename W, int V, int N> static cudaError_t norm_backward_rows(const Launch &L, const NormCall &c, int *parts) {
+  NormShape s = norm_shape(c.D.d, N, NORM_GRAD_VALUES(N));
+  const bool post = c.D.flags & PM_NORM_POST, pre = c.D.flags & PM_NORM_PRE, gate = c.D.gate != PM_NORM_GATE_NONE;
+  const int row = ((pre ? 2 : 0) + (post || gate ? 1 : 0) + (c.dr ? 1 : 0)) * N / V;
+  s.slots = N / 2;
+  if (V > 1 && row) norm_ring(s, N / 2, row);
+  *parts = norm_parts(s, c.T, L.n_sm);
+  if constexpr (V > 1) return norm_go_mode<E, W, V, N, true>(L, *parts, s, c);
+  else return norm_go<E, W, V, N, false, NORM_ANY, true>(L, *parts, s, c);
 }
 template <typename E, typename W, int V> static cudaError_t norm_backward(const Launch &L, const NormCall &c) {
-  NormShape s = norm_shape(c.D.d, NORM_GRAD_THREADS);
   int parts = 0;
   float *channel = c.D.gate == PM_NORM_GATE_CHANNEL ? c.dgate : nullptr;
   if (c.T) {  // (no rows: the sums alone, zeros)
-    const bool post = c.D.flags & PM_NORM_POST, pre = c.D.flags & PM_NORM_PRE, gate = c.D.gate != PM_NORM_GATE_NONE;
-    const int row = ((pre ? 2 : 0) + (post || gate ? 1 : 0) + (c.dr ? 1 : 0)) * NORM_VALUES / V;
-    s.slots = 4;
-    if (V > 1 && row) norm_ring(s, 4, row);
-    parts = norm_parts(s, c.T, L.n_sm);
     cudaError_t e;
-    if constexpr (V > 1) e = norm_go_mode<E, W, V, true>(L, parts, s, c);
-    else e = norm_go<E, W, V, false, NORM_ANY, true>(L, parts, s, c);
+    if constexpr (V == 8) e = norm_backward_rows<E, W, V, 16>(L, c, &parts);  // (norm_values)
+    else e = norm_backward_rows<E, W, V, 8>(L, c, &parts);
     if (e != cudaSuccess) return e;
   }
   if (!c.dw_pre && !c.dw_post && !channel) return cudaSuccess;
-  return pm_launch(L, k_norm_sum_parts, dim3((c.D.d + 31) / 32, 3), 256, 0, (const float *)c.parts, parts, c.D.d, c.dw_pre, c.dw_post, channel);
+  return pm_launch(L, k_norm_sum_parts, dim3((c.D.d + 31) / 32, 3), 1024, 0, (const float *)c.parts, parts, c.D.d, c.dw_pre, c.dw_post, channel);
 }
 
 #define NORM_TYPES(F)                                                                                                      \

@@ -336,8 +336,8 @@ __global__ void __launch_bounds__(256, rows_ctas(V, KB, SPREAD, DOT)) k_rows(Row
           if (V == 1 && k >= (int)K) break;
           if (!SPREAD || DOT) {
             const VecF<V> g = vf_widen<E, V>(r[k][j]);
-            if (DOT) vf_dot<V>(dot[k], g, f);
-            if (!SPREAD) vf_fma<V>(acc, g, wk[k]);
+            if (DOT) vf_dot_add<V>(dot[k], g, f);
+            if (!SPREAD) vf_add<V>(acc, g, wk[k]);
           }
           if (SPREAD && pos[k] != PM_ROWS_NONE)
             pm_store<E, V>(out + (size_t)pos[k] * c.D.rows_stride + (size_t)v * V, w ? vf_narrow<E, V>(vf_mul<V>(f, wk[k])) : s[j]);

@@ -75,7 +75,7 @@ template <typename E, int V> __device__ __forceinline__ Raw<E, V> pm_narrow(cons
   return r;
 }
 
-// eight f32 values as four pairs: one instruction works on a pair (each value rounded as by the scalar one)
+// one instruction works on a pair (each value rounded as by the scalar one)
 __device__ __forceinline__ uint64_t pm_mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -86,38 +86,6 @@ __device__ __forceinline__ uint64_t pm_add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-struct F8 {
-  uint64_t p[4];
-  __device__ __forceinline__ static F8 all(float v) {
-    const uint64_t b = pm_pack2(v, v);
-    return {{b, b, b, b}};
-  }
-  __device__ __forceinline__ float sum() const {
-    const uint64_t a = pm_add2(pm_add2(p[0], p[1]), pm_add2(p[2], p[3]));
-    float x, y;
-    pm_unpack2(a, x, y);
-    return __fadd_rn(x, y);
-  }
-};
-__device__ __forceinline__ F8 operator*(const F8 &a, const F8 &b) {
-  return {{pm_mul2(a.p[0], b.p[0]), pm_mul2(a.p[1], b.p[1]), pm_mul2(a.p[2], b.p[2]), pm_mul2(a.p[3], b.p[3])}};
-}
-__device__ __forceinline__ F8 operator*(const F8 &a, float s) { return a * F8::all(s); }
-__device__ __forceinline__ F8 operator+(const F8 &a, const F8 &b) {
-  return {{pm_add2(a.p[0], b.p[0]), pm_add2(a.p[1], b.p[1]), pm_add2(a.p[2], b.p[2]), pm_add2(a.p[3], b.p[3])}};
-}
-__device__ __forceinline__ F8 fma8(const F8 &a, const F8 &b, const F8 &c) {
-  return {{pm_fma2(a.p[0], b.p[0], c.p[0]), pm_fma2(a.p[1], b.p[1], c.p[1]), pm_fma2(a.p[2], b.p[2], c.p[2]), pm_fma2(a.p[3], b.p[3], c.p[3])}};
-}
-__device__ __forceinline__ F8 fma8(const F8 &a, float s, const F8 &c) { return fma8(a, F8::all(s), c); }
-// the sum of a b over the eight
-__device__ __forceinline__ float dot8(const F8 &a, const F8 &b) {
-  const uint64_t s = pm_fma2(a.p[3], b.p[3], pm_fma2(a.p[2], b.p[2], pm_fma2(a.p[1], b.p[1], pm_mul2(a.p[0], b.p[0]))));
-  float x, y;
-  pm_unpack2(s, x, y);
-  return __fadd_rn(x, y);
-}
-
 // V f32 values, in pairs where there are any
 template <int V> struct VecF {
   uint64_t p[V / 2];
@@ -162,7 +130,7 @@ template <int V> __device__ __forceinline__ VecF<V> vf_mul(const VecF<V> &a, flo
   }
   return f;
 }
-template <int V> __device__ __forceinline__ void vf_fma(VecF<V> &acc, const VecF<V> &a, float s) {
+template <int V> __device__ __forceinline__ void vf_add(VecF<V> &acc, const VecF<V> &a, float s) {
   if constexpr (V == 1) acc.p[0] = __fmaf_rn(a.p[0], s, acc.p[0]);
   else {
 #pragma unroll
@@ -173,7 +141,7 @@ template <int V> __device__ __forceinline__ void vf_fma(VecF<V> &acc, const VecF
 template <int V> struct DotT { using T = uint64_t; };
 template <> struct DotT<1> { using T = float; };
 template <int V> using DotOf = typename DotT<V>::T;
-template <int V> __device__ __forceinline__ void vf_dot(DotOf<V> &acc, const VecF<V> &a, const VecF<V> &b) {
+template <int V> __device__ __forceinline__ void vf_dot_add(DotOf<V> &acc, const VecF<V> &a, const VecF<V> &b) {
   if constexpr (V == 1) acc = __fmaf_rn(a.p[0], b.p[0], acc);
   else {
 #pragma unroll
@@ -185,4 +153,37 @@ __device__ __forceinline__ float vf_sum(uint64_t v) {
   float a, b;
   pm_unpack2(v, a, b);
   return __fadd_rn(a, b);
+}
+// the arithmetic of whole vectors (pairs)
+template <int N> __device__ __forceinline__ VecF<N> vf_all(float v) {
+  VecF<N> f;
+#pragma unroll
+  for (int i = 0; i < N / 2; i++) f.p[i] = pm_pack2(v, v);
+  return f;
+}
+template <int N> __device__ __forceinline__ VecF<N> operator*(const VecF<N> &a, const VecF<N> &b) {
+  VecF<N> f;
+#pragma unroll
+  for (int i = 0; i < N / 2; i++) f.p[i] = pm_mul2(a.p[i], b.p[i]);
+  return f;
+}
+template <int N> __device__ __forceinline__ VecF<N> operator*(const VecF<N> &a, float s) { return vf_mul<N>(a, s); }
+template <int N> __device__ __forceinline__ VecF<N> operator+(const VecF<N> &a, const VecF<N> &b) {
+  VecF<N> f;
+#pragma unroll
+  for (int i = 0; i < N / 2; i++) f.p[i] = pm_add2(a.p[i], b.p[i]);
+  return f;
+}
+template <int N> __device__ __forceinline__ VecF<N> vf_fma(const VecF<N> &a, const VecF<N> &b, const VecF<N> &c) {
+  VecF<N> f;
+#pragma unroll
+  for (int i = 0; i < N / 2; i++) f.p[i] = pm_fma2(a.p[i], b.p[i], c.p[i]);
+  return f;
+}
+template <int N> __device__ __forceinline__ VecF<N> vf_fma(const VecF<N> &a, float s, const VecF<N> &c) { return vf_fma(a, vf_all<N>(s), c); }
+template <int N> __device__ __forceinline__ float vf_dot(const VecF<N> &a, const VecF<N> &b) {
+  uint64_t s = pm_mul2(a.p[0], b.p[0]);
+#pragma unroll
+  for (int i = 1; i < N / 2; i++) s = pm_fma2(a.p[i], b.p[i], s);
+  return vf_sum(s);
 }
