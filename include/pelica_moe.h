@@ -478,6 +478,13 @@ PM_API int32_t pm_stack_forward(pm_stack *stack, const float *x, int32_t T, floa
  * was created is picked up by the next pm_stack_forward. */
 PM_API int32_t pm_stack_set_mode(pm_stack *stack, int32_t mode);
 PM_API int32_t pm_stack_decode_kernel_available(pm_stack *stack);
+/* A model's own norms around layer `layer` of the stack (no counterpart in the reference, as pm_block_norm):
+ *   xn = x or, with PM_NORM_PRE, its norm; f = moe(xn); x = alpha x + beta gate p, p = f or, with PM_NORM_POST, its norm.
+ * norm: dtype and wtype f32, d the stack's, gate PM_NORM_GATE_NONE or _CHANNEL, strides 0. w_pre, w_post, gate: [d] f32, host or
+ * device memory, copied (w_pre, w_post NULL: ones). norm NULL: the plain form (x / rms(x), x += f) again. A stack with norms runs in
+ * the general kernels, its steps fused with pm_block_norm's; a failed call leaves the layer as it was. */
+PM_API int32_t pm_stack_set_norm(pm_stack *stack, int32_t layer, const pm_norm_desc *norm, const float *w_pre,
+                                 const float *w_post, const float *gate);
 /* PM_OK, or PM_ERR_TIMEOUT when a device-side wait of an earlier call gave up
  * (synchronises the context's stream) */
 PM_API int32_t pm_stack_status(pm_stack *stack);

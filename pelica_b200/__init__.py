@@ -142,6 +142,7 @@ ABI = {
     "pm_stack_forward": (C.c_int32, [_VP, _VP, C.c_int32, _VP]),
     "pm_stack_set_mode": (C.c_int32, [_VP, C.c_int32]),
     "pm_stack_decode_kernel_available": (C.c_int32, [_VP]),
+    "pm_stack_set_norm": (C.c_int32, [_VP, C.c_int32, C.POINTER(NormDesc), _VP, _VP, _VP]),
     "pm_stack_status": (C.c_int32, [_VP]),
     "pm_layer_fill_synthetic": (C.c_int32, [_VP, C.c_uint64, C.c_float, C.c_float, C.c_float]),
     "pm_layer_get_expert_bias": (C.c_int32, [_VP, C.c_int32, _VP, _VP, _VP]),
@@ -646,6 +647,20 @@ class Stack:
 
     def forward_dev(self, x: DevBuf, T: int, out: DevBuf):
         _check(self.lib.pm_stack_forward(self.h, x.ptr, T, out.ptr))
+
+    def set_norm(self, layer: int, w_pre=None, w_post=None, gate=None, pre: bool = True, post: bool = False, alpha: float = 1.0,
+                 beta: float = 1.0, eps_pre: float = 1e-6, eps_post: float = 1e-6, offset_pre: float = 0.0, offset_post: float = 0.0):
+        """The model's norms around a layer: x <- alpha x + beta gate post(moe(pre(x))). Weights: [d] f32 arrays or DevBufs, copied."""
+        w = [None if a is None else _f32(a) for a in (w_pre, w_post, gate)]
+        for a in w:
+            assert a is None or (a.nbytes >= 4 * self.d if isinstance(a, DevBuf) else a.size == self.d)
+        desc = NormDesc(synth.F32, synth.F32, self.d, PM_NORM_POST * bool(post) | PM_NORM_PRE * bool(pre),
+                        NORM_GATES["none" if gate is None else "channel"], eps_post, eps_pre, offset_post, offset_pre, alpha, beta)
+        _check(self.lib.pm_stack_set_norm(self.h, layer, C.byref(desc), *(_ptr(a) for a in w)))
+
+    def clear_norm(self, layer: int):
+        """The plain form around a layer again: x <- x + moe(x / rms(x))."""
+        _check(self.lib.pm_stack_set_norm(self.h, layer, None, None, None, None))
 
     def set_mode(self, general_only: bool):
         """True: always the general kernels; False: one-token calls use the persistent decode kernel."""

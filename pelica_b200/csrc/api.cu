@@ -1991,7 +1991,25 @@ struct pm_stack {
   bool fault_next = false;         // pm_debug_stack_fault_next_call
   std::vector<uint64_t> seen_gen;  // the layers' generation counters when their pointers were last snapshot
   uint64_t seen_dispatch = 0;      // the context's dispatch_gen that the graphs were recorded under
+  // norms of the model's own (pm_stack_set_norm): per layer; empty while the stack has none
+  struct Norm {
+    pm_norm_desc D;
+    float *buf;                          // null: the plain form
+    const float *w_pre, *w_post, *gate;  // in buf, or null
+  };
+  std::vector<Norm> norms;
 };
+
+// the plain form around a layer, x / rms(x) and x += f, as a norm
+static pm_stack::Norm stack_plain_norm(const pm_stack *s) {
+  pm_stack::Norm n = {};
+  n.D.dtype = n.D.wtype = PM_TYPE_F32;
+  n.D.d = s->layers[0]->dev.desc.d;
+  n.D.flags = PM_NORM_PRE;
+  n.D.eps_pre = s->eps;
+  n.D.alpha = n.D.beta = 1.0f;
+  return n;
+}
 
 // (re)writes the decode kernel's per-layer pointer table from the layers' current state
 static int32_t stack_fill_mega_layers(pm_stack *s) {
@@ -2107,6 +2125,7 @@ extern "C" int32_t pm_stack_destroy(pm_stack *s) {
   cudaSetDevice(s->ctx->device);
   cudaStreamSynchronize(s->ctx->stream);
   stack_drop_graphs(s);
+  for (pm_stack::Norm &n : s->norms) cudaFree(n.buf);
   if (s->mega_layers) cudaFree(s->mega_layers);
   if (s->mega_buf) cudaFree(s->mega_buf);
   if (s->mega_io) cudaFree(s->mega_io);
@@ -2119,7 +2138,7 @@ extern "C" int32_t pm_stack_set_mode(pm_stack *s, int32_t mode) {
   s->mode = mode;
   return PM_OK;
 }
-extern "C" int32_t pm_stack_decode_kernel_available(pm_stack *s) { return s && s->mega_ok ? 1 : 0; }
+extern "C" int32_t pm_stack_decode_kernel_available(pm_stack *s) { return s && s->mega_ok && s->norms.empty() ? 1 : 0; }
 
 extern "C" int32_t pm_stack_trace(pm_stack *s, int64_t *out, int32_t capacity) {
   if (!s || !s->mega_ok) return fail(PM_ERR_STATE, "pm_stack_trace: no decode kernel for this stack");
@@ -2206,6 +2225,111 @@ static int32_t stack_forward_mega(pm_stack *s, const float *x, float *x_out) {
   return PM_OK;
 }
 
+extern "C" int32_t pm_stack_set_norm(pm_stack *s, int32_t layer, const pm_norm_desc *norm, const float *w_pre, const float *w_post,
+                                     const float *gate) {
+  static const char *call = "pm_stack_set_norm";
+  if (!s) return fail(PM_ERR_INVALID, "%s: null stack", call);
+  const size_t L = s->layers.size();
+  if (layer < 0 || (size_t)layer >= L) return fail(PM_ERR_INVALID, "%s: layer %d of %zu", call, layer, L);
+  const size_t d = (size_t)s->layers[0]->dev.desc.d;
+  pm_stack::Norm n = stack_plain_norm(s);
+  CU(cudaSetDevice(s->ctx->device));
+  if (norm) {
+    TRY(norm_desc_check(call, norm, 1, &n.D));
+    if (n.D.dtype != PM_TYPE_F32 || n.D.wtype != PM_TYPE_F32) return fail(PM_ERR_UNSUPPORTED, "%s: a stack's stream is f32", call);
+    if ((size_t)n.D.d != d) return fail(PM_ERR_INVALID, "%s: d=%d, the stack has %zu", call, n.D.d, d);
+    if (n.D.gate == PM_NORM_GATE_TOKEN) return fail(PM_ERR_UNSUPPORTED, "%s: a gate of the tokens", call);
+    if (n.D.gate == PM_NORM_GATE_CHANNEL && !gate) return fail(PM_ERR_INVALID, "%s: gate is null", call);
+    if (norm->x_stride || norm->f_stride || norm->r_stride || norm->n_stride) return fail(PM_ERR_INVALID, "%s: strides must be 0", call);
+    n.D.x_stride = n.D.f_stride = n.D.r_stride = n.D.n_stride = 0;
+    CU(cudaMalloc(&n.buf, 3 * al(d * 4)));
+    const float *from[3] = {n.D.flags & PM_NORM_PRE ? w_pre : nullptr, n.D.flags & PM_NORM_POST ? w_post : nullptr,
+                            n.D.gate == PM_NORM_GATE_CHANNEL ? gate : nullptr};
+    const float **to[3] = {&n.w_pre, &n.w_post, &n.gate};
+    for (int i = 0; i < 3; i++) {
+      if (!from[i]) continue;
+      float *p = (float *)((uint8_t *)n.buf + i * al(d * 4));
+      const cudaError_t e = cudaMemcpyAsync(p, from[i], d * 4, cudaMemcpyDefault, s->ctx->stream);
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        cudaStreamSynchronize(s->ctx->stream);
+        cudaFree(n.buf);
+        return fail(PM_ERR_CUDA, "%s: %s", call, cudaGetErrorString(e));
+      }
+      *to[i] = p;
+    }
+  }
+  CU(cudaStreamSynchronize(s->ctx->stream));  // nothing uses what is replaced, and the copies are done
+  if (s->norms.empty()) {
+    if (!norm) return PM_OK;
+    s->norms.assign(L, stack_plain_norm(s));
+  }
+  stack_drop_graphs(s);
+  if (s->norms[layer].buf) CU(cudaFree(s->norms[layer].buf));
+  s->norms[layer] = n;
+  bool any = false;
+  for (const pm_stack::Norm &q : s->norms) any = any || q.buf;
+  if (!any) s->norms.clear();
+  return PM_OK;
+}
+
+// the step between layers: the residual stream takes layer i - 1's output f (i > 0), and is normed for layer i (i < layers)
+static int32_t stack_norm_step(pm_stack *s, size_t i, int T, float *x, float *f, float *xn) {
+  NormCall c = {};
+  c.T = T;
+  c.D = stack_plain_norm(s).D;
+  c.D.flags = 0;
+  c.inv_d = 1.0f / (float)c.D.d;
+  c.D.x_stride = c.D.f_stride = c.D.r_stride = c.D.n_stride = c.D.d;
+  c.x = x;
+  if (i > 0) {
+    const pm_stack::Norm &n = s->norms[i - 1];
+    c.f = f;
+    c.r = x;
+    c.D.flags |= n.D.flags & PM_NORM_POST;
+    c.D.gate = n.D.gate;
+    c.D.alpha = n.D.alpha;
+    c.D.beta = n.D.beta;
+    c.D.eps_post = n.D.eps_post;
+    c.D.offset_post = n.D.offset_post;
+    c.w_post = n.w_post;
+    c.gate = n.gate;
+  }
+  if (i < s->layers.size() && (s->norms[i].D.flags & PM_NORM_PRE)) {
+    const pm_stack::Norm &n = s->norms[i];
+    c.D.flags |= PM_NORM_PRE;
+    c.D.eps_pre = n.D.eps_pre;
+    c.D.offset_pre = n.D.offset_pre;
+    c.w_pre = n.w_pre;
+    c.n = xn;
+  }
+  if (!c.r && !c.n) return PM_OK;
+  c.vec = norm_vec(c.D, {x, c.f, c.n});
+  PROF(s->ctx, PH_NORM);
+  CU(launch_block_norm(s->ctx->launch(), c));
+  return PM_OK;
+}
+
+// every layer over the residual stream x, in place; xn, f: a layer's input and (stacks with norms) output; workspace from here on
+static int32_t stack_layers(pm_stack *s, int T, float *x, float *xn, float *f) {
+  pm_ctx *c = s->ctx;
+  const size_t mark = c->ws_off, L = s->layers.size();
+  for (size_t i = 0; i < L; i++) {
+    pm_layer *ly = s->layers[i];
+    c->ws_off = mark;
+    Scratch S;
+    scratch_carve(c, ly->dev.desc, T, S);
+    if (!s->norms.empty()) {
+      TRY(stack_norm_step(s, i, T, x, f, xn));
+      TRY(dev_forward(ly, s->norms[i].D.flags & PM_NORM_PRE ? xn : x, T, f, false, S));
+      continue;
+    }
+    if (i == 0) { PROF(c, PH_NORM); launch_rmsnorm(c->launch(), x, T, ly->dev.desc.d, s->eps, xn); }
+    TRY(dev_forward(ly, xn, T, x, true, S, i + 1 < L ? xn : nullptr, s->eps));
+  }
+  return s->norms.empty() ? PM_OK : stack_norm_step(s, L, T, x, f, xn);
+}
+
 extern "C" int32_t pm_stack_forward(pm_stack *s, const float *x, int32_t T, float *x_out) {
   if (!s || !x || !x_out) return fail(PM_ERR_INVALID, "pm_stack_forward: null argument");
   TRY(check_T(T));
@@ -2214,7 +2338,7 @@ extern "C" int32_t pm_stack_forward(pm_stack *s, const float *x, int32_t T, floa
   CU(cudaSetDevice(c->device));
   for (pm_layer *ly : s->layers) TRY(layer_ready(ly, true));
   TRY(stack_refresh(s));
-  if (T == 1 && s->mega_ok && s->mode == 0) return stack_forward_mega(s, x, x_out);
+  if (T == 1 && s->mega_ok && s->mode == 0 && s->norms.empty()) return stack_forward_mega(s, x, x_out);
   const int d = s->layers[0]->dev.desc.d;
   size_t n = (size_t)T * d;
   size_t need = 0;
@@ -2222,7 +2346,7 @@ extern "C" int32_t pm_stack_forward(pm_stack *s, const float *x, int32_t T, floa
     size_t b = scratch_bytes(ly->dev.desc, T);
     if (b > need) need = b;
   }
-  TRY(ws_reserve(c, need + 3 * al(n * 4)));
+  TRY(ws_reserve(c, need + (s->norms.empty() ? 3 : 4) * al(n * 4)));
   // ---- a few tokens: replay the recorded loop ----
   bool graphable = T <= 16 && !c->prof_on && !s->graph_off;
   for (pm_layer *ly : s->layers) graphable = graphable && ly->dev.desc.shared == PM_SHARED_NONE;
@@ -2247,22 +2371,13 @@ extern "C" int32_t pm_stack_forward(pm_stack *s, const float *x, int32_t T, floa
     if (!g && seen) {  // second call with this token count: record
       pm_stack::Graph q{T, c->ws, nullptr, nullptr, 0};
       CU(cudaMalloc(&q.gx, n * 4));
-      float *xn = ws_take<float>(c, n);
-      size_t mark = c->ws_off;
+      float *xn = ws_take<float>(c, n), *f = s->norms.empty() ? nullptr : ws_take<float>(c, n);
       int64_t l0 = c->launches;
       cudaGraph_t graph = nullptr;
       bool ok = cudaStreamBeginCapture(c->stream, cudaStreamCaptureModeThreadLocal) == cudaSuccess;
       int32_t rc = PM_OK;
       if (ok) {
-        size_t done = 0;
-        for (pm_layer *ly : s->layers) {
-          c->ws_off = mark;
-          Scratch S;
-          scratch_carve(c, ly->dev.desc, T, S);
-          if (done == 0) launch_rmsnorm(c->launch(), q.gx, T, d, s->eps, xn);
-          rc = dev_forward(ly, xn, T, q.gx, true, S, ++done < s->layers.size() ? xn : nullptr, s->eps);
-          if (rc != PM_OK) break;
-        }
+        rc = stack_layers(s, T, q.gx, xn, f);
         ok = cudaStreamEndCapture(c->stream, &graph) == cudaSuccess && rc == PM_OK && graph;
       }
       q.launches = c->launches - l0;
@@ -2292,17 +2407,9 @@ extern "C" int32_t pm_stack_forward(pm_stack *s, const float *x, int32_t T, floa
   }
   // residual stream: in place in x_out when it is a device pointer
   float *xc = is_device_ptr(x_out) ? x_out : ws_take<float>(c, n);
-  float *xn = ws_take<float>(c, n);
+  float *xn = ws_take<float>(c, n), *f = s->norms.empty() ? nullptr : ws_take<float>(c, n);
   if (xc != x) CU(cudaMemcpyAsync(xc, x, n * 4, cudaMemcpyDefault, c->stream));
-  size_t mark = c->ws_off;
-  for (size_t i = 0; i < s->layers.size(); i++) {
-    pm_layer *ly = s->layers[i];
-    c->ws_off = mark;
-    Scratch S;
-    scratch_carve(c, ly->dev.desc, T, S);
-    if (i == 0) { PROF(c, PH_NORM); launch_rmsnorm(c->launch(), xc, T, d, s->eps, xn); }
-    TRY(dev_forward(ly, xn, T, xc, true, S, i + 1 < s->layers.size() ? xn : nullptr, s->eps));
-  }
+  TRY(stack_layers(s, T, xc, xn, f));
   if (xc != x_out) {
     CU(cudaMemcpyAsync(x_out, xc, n * 4, cudaMemcpyDeviceToHost, c->stream));
     CU(cudaStreamSynchronize(c->stream));

@@ -1,0 +1,155 @@
+"""A model's own norms in the layer loop, and the operators run together as a host with products of its own uses them."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import pelica_b200 as pb
+from pelica_b200 import synth
+from tests.helpers import SMALL, bits_equal, tol_ok
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def tctx():
+    c = pb.Context(0, stream=torch.cuda.current_stream().cuda_stream)
+    yield c
+    c.close()
+
+
+class Buf:
+    """A torch tensor as a device buffer of the library's calls."""
+
+    def __init__(self, t):
+        self.t, self.ptr, self.nbytes = t, t.data_ptr(), t.numel() * t.element_size()
+
+
+def layers_of(ctx, cfg, n):
+    return [pb.MoeLayer(ctx, cfg).load(synth.make_weights(cfg, 30 + i)) for i in range(n)]
+
+
+NORMS = [dict(pre=True, post=True, alpha=0.5, beta=1.25, offset_pre=1.0, offset_post=1.0, gated=True), dict(pre=True, eps_pre=1e-5, alpha=1.0),
+         dict(pre=False, post=True, eps_post=1e-5)]
+
+
+def norm_weights(d, seed):
+    rng = np.random.default_rng(seed)
+    return [rng.normal(0.2, 0.3, d).astype(np.float32) for _ in range(3)]
+
+
+def by_hand(ctx, layers, d, x):
+    """The loop from the layers and the block norm."""
+    T = x.shape[0]
+    x = torch.from_numpy(x).cuda()
+    for i, layer in enumerate(layers):
+        k = dict(NORMS[i])
+        gated = k.pop("gated", False)
+        w = [torch.from_numpy(a).cuda() for a in norm_weights(d, i)]
+        xn, f = x.clone(), torch.zeros_like(x)
+        if k.get("pre"):
+            pb.BlockNorm(ctx, d, pre=True, eps_pre=k.get("eps_pre", 1e-6), offset_pre=k.get("offset_pre", 0.0)).forward(
+                T, x.data_ptr(), None, None, xn.data_ptr(), w_pre=w[0].data_ptr())
+        layer.forward_dev(Buf(xn), T, Buf(f))
+        out = torch.empty_like(x)
+        pb.BlockNorm(ctx, d, pre=False, post=k.get("post", False), gate="channel" if gated else "none", alpha=k.get("alpha", 1.0),
+                     beta=k.get("beta", 1.0), eps_post=k.get("eps_post", 1e-6), offset_post=k.get("offset_post", 0.0)).forward(
+            T, x.data_ptr(), f.data_ptr(), out.data_ptr(), w_post=w[1].data_ptr(), gate=w[2].data_ptr() if gated else None)
+        x = out
+    ctx.sync()
+    return x.cpu().numpy()
+
+
+@pytest.mark.parametrize("name", ["c2", "c3", "c4"])
+def test_norms_of_a_stack(tctx, name):
+    cfg = SMALL[name]
+    layers = layers_of(tctx, cfg, 3)
+    st = pb.Stack(tctx, layers)
+    had = st.decode_kernel
+    xs = {T: synth.make_activations(T, cfg.d, 50 + T) for T in (1, 5, 40)}
+    plain = {T: st.forward(x).copy() for T, x in xs.items()}
+    for i, k in enumerate(NORMS):
+        k = dict(k)
+        w = norm_weights(cfg.d, i)
+        gate = w[2] if k.pop("gated", False) else None
+        st.set_norm(i, w[0], w[1], gate, **k)
+    assert not st.decode_kernel
+    for T, x in xs.items():
+        want = by_hand(tctx, layers, cfg.d, x)
+        for _ in range(3):  # the loop, its recording, a replay
+            assert bits_equal(st.forward(x), want), T
+    st.clear_norm(1)
+    st.set_norm(0)  # unit weights: the plain form by the other kernel
+    st.clear_norm(2)
+    for T, x in xs.items():
+        if name == "c3":  # (int8 layers: a value may round the other way)
+            assert tol_ok(st.forward(x), plain[T])
+    st.clear_norm(0)
+    assert st.decode_kernel == had
+    for T, x in xs.items():
+        assert bits_equal(st.forward(x), plain[T])
+    st.close()
+    for layer in layers:
+        layer.close()
+
+
+def test_refusals_of_stack_norms(tctx):
+    cfg = SMALL["c3"]
+    layers = layers_of(tctx, cfg, 1)
+    st = pb.Stack(tctx, layers)
+    good = dict(dtype=synth.F32, wtype=synth.F32, d=cfg.d, flags=3, gate=0, eps_pre=1e-6, eps_post=1e-6, alpha=1.0, beta=1.0)
+    x = synth.make_activations(4, cfg.d, 9)
+    before = st.forward(x).copy()
+
+    def call(layer=0, **change):
+        return st.lib.pm_stack_set_norm(st.h, layer, C.byref(pb.NormDesc(**{**good, **change})), None, None, None)
+
+    for got in (call(1), call(-1), call(d=cfg.d + 32), call(gate=1), call(x_stride=cfg.d), call(eps_pre=-1.0), call(flags=8)):
+        assert got == -1
+    for got in (call(dtype=synth.BF16), call(gate=2)):
+        assert got == -2
+    assert st.lib.pm_stack_set_norm(None, 0, None, None, None, None) == -1
+    st.clear_norm(0)
+    assert bits_equal(st.forward(x), before)
+    st.close()
+    layers[0].close()
+
+
+@pytest.mark.parametrize("name, T", [("c2", 1), ("c2", 37), ("c3", 20), ("c4", 200)])
+def test_the_operators_together(tctx, name, T):
+    """norm -> route -> dispatch -> experts on the rows -> collect beside the shared expert -> norm: the layer's own output."""
+    cfg = SMALL[name]
+    layer = pb.MoeLayer(tctx, cfg).load(synth.make_weights(cfg, 3))
+    d, K, E = cfg.d, cfg.top_k, cfg.n_exp
+    x = torch.from_numpy(synth.make_activations(T, d, 11)).cuda()
+    new = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t, device="cuda")  # noqa: E731
+    norm = pb.BlockNorm(tctx, d, post=True, pre=True, alpha=0.75)
+    xn, out, nxt = new(T, d), new(T, d), new(T, d)
+    pb.BlockNorm(tctx, d).forward(T, x.data_ptr(), None, None, xn.data_ptr())
+    tctx.sync()
+    ids, w = layer.route(xn.cpu().numpy())
+    ids_d, w_d = torch.from_numpy(ids.astype(np.int32)).cuda(), torch.from_numpy(w).cuda()
+    rows_op = pb.Rows(tctx, d, K, E)
+    R = rows_op.bound(T)
+    rows, outs = new(R, d), new(R, d)
+    offset, count, pos = new(E + 1, t=torch.int32), new(E, t=torch.int32), new(T, K, t=torch.int32)
+    expert, weight = new(R, t=torch.int32), new(R)
+    plan = rows_op.plan(R, offset.data_ptr(), count.data_ptr(), pos.data_ptr(), row_expert=expert.data_ptr(), row_weight=weight.data_ptr())
+    rows_op.dispatch(T, ids_d.data_ptr(), plan, xn.data_ptr(), rows.data_ptr(), w=w_d.data_ptr(), scale=False)
+    pb._check(layer.lib.pm_experts_rows(layer.h, rows.data_ptr(), R, expert.data_ptr(), weight.data_ptr(), outs.data_ptr()))
+    shared = torch.from_numpy(layer.shared(xn.cpu().numpy())).cuda() if cfg.shared else None
+    folded = cfg.weight_fold == synth.FOLD_BEFORE_DOWN  # the experts have applied the weights already
+    y = new(T, d)
+    rows_op.collect(T, plan, outs.data_ptr(), y.data_ptr(), w=None if folded else w_d.data_ptr(), add=None if shared is None else shared.data_ptr())
+    norm.forward(T, x.data_ptr(), y.data_ptr(), out.data_ptr(), nxt.data_ptr())
+    tctx.sync()
+    want = layer.forward(xn.cpu().numpy())
+    assert tol_ok(y.cpu().numpy(), want)  # (the order of the shared expert's addition differs)
+    f, x64 = y.cpu().double(), x.cpu().double()
+    r = 0.75 * x64 + f / (f.pow(2).mean(1, keepdim=True) + 1e-6).sqrt()
+    size = float(r.abs().max()) + float(x64.abs().max())  # of the terms; 64 roundings of 2^-24 for each of the two norms
+    assert float((out.cpu().double() - r).abs().max()) <= 64 * 2.0 ** -24 * 2 * size
+    s = (r.pow(2).mean(1, keepdim=True) + 1e-6).sqrt()
+    assert float(((nxt.cpu().double() - r / s) * s).abs().max()) <= 128 * 2.0 ** -24 * 2 * size
+    layer.close()
