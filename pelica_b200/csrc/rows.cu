@@ -76,33 +76,35 @@ __device__ __forceinline__ void rows_write_pad(const RowsCall &c, uint32_t e, ui
   if (c.pl.row_weight) c.pl.row_weight[row] = 0.0f;
 }
 
-// zeros in rows [from, to), by all threads of the CTA
-template <typename E, int V> __device__ __forceinline__ void rows_zero(const RowsCall &c, E *rows, uint32_t from, uint32_t to) {
-  const float z[V] = {};
-  const Raw<E, V> zero = pm_narrow<E, V>(z);
+// a row of zeros, by all threads of the CTA
+template <typename E, int V> __device__ __forceinline__ void rows_zero(const RowsCall &c, E *rows, uint32_t r) {
+  const Raw<E, V> zero = vf_narrow<E, V>(vf_zero<V>());
   const uint32_t dv = (uint32_t)c.D.d / V;
-  for (uint32_t r = from; r < to; r++)
-    for (uint32_t v = threadIdx.x; v < dv; v += blockDim.x) pm_store<E, V>(rows + (size_t)r * c.D.rows_stride + (size_t)v * V, zero);
+  for (uint32_t v = threadIdx.x; v < dv; v += blockDim.x) pm_store<E, V>(rows + (size_t)r * c.D.rows_stride + (size_t)v * V, zero);
 }
 
 // ---------------------------------------------------------------------------
 // plan and rows of a few pairs in one launch
 // ---------------------------------------------------------------------------
-// Grid (token, slab of 256 vectors). Every CTA sorts all pairs for itself - at most PM_ROWS_SMALL_PAIRS, in shared memory -
-// and copies its piece of its token: no CTA waits for another.
+// Grid (token, slab of 256 vectors), and as many CTAs without a token as spread the padding over the GPU. Every CTA sorts all pairs
+// for itself - at most PM_ROWS_SMALL_PAIRS, in shared memory - and copies its piece of its token: no CTA waits for another.
+#define ROWS_PAD_CTAS 256  // at least, where groups are padded
+#define ROWS_PAD_LIST PM_MAX_EXPERTS  // padding rows of one CTA: no group has ROWS_PAD_CTAS of them
+static_assert(ROWS_PAD_CTAS >= PM_ROWS_MAX_ALIGN, "a CTA has one padding row of a group");
 template <typename E, int V>
 __global__ void __launch_bounds__(256) k_rows_dispatch_small(RowsCall c, const uint32_t *__restrict__ ids, const float *__restrict__ w, bool scale,
                                                              const E *__restrict__ x, E *__restrict__ rows) {
   pm_pdl();
   __shared__ uint16_t le[PM_ROWS_SMALL_PAIRS];
   __shared__ uint32_t cnt[PM_MAX_EXPERTS], off[PM_MAX_EXPERTS + 1], part[8];
-  __shared__ uint32_t at[PM_MAX_TOPK];
+  __shared__ uint32_t at[PM_MAX_TOPK], pad[ROWS_PAD_LIST], n_pad;
   __shared__ float ws[PM_MAX_TOPK];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = c.D.top_k;
   const uint32_t P = (uint32_t)c.T * K, t = blockIdx.x, p0 = t * K, dv = (uint32_t)c.D.d / V;
   const uint32_t v0 = blockIdx.y * 256 + tid;
   Raw<E, V> mine;
-  if (x && v0 < dv) mine = pm_load<E, V>(x + (size_t)t * c.D.x_stride + (size_t)v0 * V);
+  const bool live = x && t < (uint32_t)c.T;
+  if (live && v0 < dv) mine = pm_load<E, V>(x + (size_t)t * c.D.x_stride + (size_t)v0 * V);
   for (int e = tid; e < PM_MAX_EXPERTS; e += 256) cnt[e] = 0;
   __syncthreads();
   for (uint32_t p = tid; p < P; p += 256) {
@@ -132,13 +134,21 @@ __global__ void __launch_bounds__(256) k_rows_dispatch_small(RowsCall c, const u
     }
     if (tid == 0) c.pl.offset[c.D.n_local] = off[c.D.n_local];
   }
-  if (c.D.align > 1)
-    for (uint32_t e = cta; e < (uint32_t)c.D.n_local; e += n_cta) {
+  if (c.D.align > 1) {  // padding row r is CTA r % n_cta's
+    if (tid == 0) n_pad = 0;
+    __syncthreads();
+    for (uint32_t e = tid; e < (uint32_t)c.D.n_local; e += 256) {
       const uint32_t from = off[e] + cnt[e], to = off[e + 1];
-      if (from + tid < to) rows_write_pad(c, e, from + tid);  // (less than the alignment, 256 at most)
-      if (x) rows_zero<E, V>(c, rows, from, to);
+      for (uint32_t r = from + (cta + n_cta - from % n_cta) % n_cta; r < to; r += n_cta) {
+        rows_write_pad(c, e, r);
+        if (x) pad[atomicAdd(&n_pad, 1u)] = r;
+      }
     }
-  if (!x) return;
+    __syncthreads();
+    if (x)
+      for (uint32_t i = 0; i < n_pad; i++) rows_zero<E, V>(c, rows, pad[i]);
+  }
+  if (!live) return;
   __syncthreads();
   for (uint32_t v = v0; v < dv; v += gridDim.y * 256) {
     if (v != v0) mine = pm_load<E, V>(x + (size_t)t * c.D.x_stride + (size_t)v * V);
@@ -267,7 +277,7 @@ __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS
 //   SPREAD   out[pos] = w src[t]                         otherwise   out[t] = add[t] + sum_k w rows[pos]
 //   DOT      dw[t][k] = <rows[pos], src[t]>
 // G: a power of two, 256 at most (a CTA); grid.y cuts the rows of a few tokens without DOT further. Behind the tokens' CTAs
-// (SPREAD), one an expert for the padding of its group. KB: K rounded up to one of five (10 pairs in a kernel for 16: 147 us instead of 126
+// (SPREAD), some for each expert's padding. KB: K rounded up to one of five (10 pairs in a kernel for 16: 147 us instead of 126
 // for 8192 x 2048 bf16 with dot products). Rows that do not start on 16 bytes go value by value, two
 // values of a row a step and 32 warps an SM (8000 x 1001 f16 with dot products, 5 pairs: 74 us; one value a step 81, four values and 8 warps
 // 112), at about half of the speed of 16-byte words.
@@ -284,10 +294,10 @@ __global__ void __launch_bounds__(256, rows_ctas(V, KB, SPREAD, DOT)) k_rows(Row
   const int tid = threadIdx.x;
   const uint32_t dv = (uint32_t)c.D.d / V, K = c.D.top_k;
   if (SPREAD && blockIdx.x >= token_ctas) {
-    const uint32_t e = blockIdx.x - token_ctas;
     if (blockIdx.y) return;
-    const uint32_t from = c.pl.offset[e] + c.pl.count[e], to = c.pl.offset[e + 1];
-    rows_zero<E, V>(c, out, from, (uint32_t)min((int64_t)to, c.pl.max_rows));
+    const uint32_t e = (blockIdx.x - token_ctas) % c.D.n_local, s = (blockIdx.x - token_ctas) / c.D.n_local;
+    const uint32_t to = (uint32_t)min((int64_t)c.pl.offset[e + 1], c.pl.max_rows);
+    for (uint32_t r = c.pl.offset[e] + c.pl.count[e] + s; r < to; r += (gridDim.x - token_ctas) / c.D.n_local) rows_zero<E, V>(c, out, r);
     return;
   }
   const uint32_t t = blockIdx.x * (256 / G) + tid / G;
@@ -389,7 +399,12 @@ static uint32_t rows_vectors(const RowsCall &c) { return c.vec ? (uint32_t)c.D.d
 template <typename E, int V, int KB, bool SPREAD, bool DOT>
 static cudaError_t rows_go(const Launch &L, const RowsCall &c, const float *w, const void *src, const void *rows, const void *add, void *out,
                            float *dw) {
-  const uint32_t dv = rows_vectors(c), pad = SPREAD && c.D.align > 1 ? (uint32_t)c.D.n_local : 0;
+  const uint32_t dv = rows_vectors(c);
+  uint32_t pad = 0;  // CTAs of the padding: two an SM, a group's rows cut as often as that takes
+  if (SPREAD && c.D.align > 1) {
+    const uint32_t cuts = 2u * L.n_sm / c.D.n_local;
+    pad = c.D.n_local * (cuts < 1 ? 1 : cuts < (uint32_t)c.D.align - 1 ? cuts : c.D.align - 1);
+  }
   int G = 4;
   while (G < 256 && (uint32_t)G < dv && (G < 32 || (SPREAD && !DOT) || (int64_t)c.T * G < (int64_t)32 * 32 * L.n_sm)) G *= 2;
   const uint32_t ctas = ((uint32_t)c.T * G + 255) / 256;
@@ -412,9 +427,11 @@ static cudaError_t rows_k(const Launch &L, const RowsCall &c, const float *w, co
 
 template <typename E, int V>
 static cudaError_t dispatch_small(const Launch &L, const RowsCall &c, const uint32_t *ids, const float *w, bool scale, const void *x, void *rows) {
-  // (a call without tokens or rows still writes its offsets)
-  const uint32_t slabs = x && c.T ? (rows_vectors(c) + 255) / 256 : 1;
-  return pm_launch(L, k_rows_dispatch_small<E, V>, dim3(c.T > 0 ? c.T : 1, slabs), 256, 0, c, ids, w, scale, (const E *)(c.T ? x : nullptr), (E *)rows);
+  // (a call without tokens or rows still writes its offsets; slabs: what eight CTAs an SM hold, each CTA sorts)
+  uint32_t ctas = c.T > 0 ? c.T : 1, slabs = x && c.T ? (rows_vectors(c) + 255) / 256 : 1;
+  if (slabs > 8u * L.n_sm / ctas) slabs = 8u * L.n_sm / ctas > 1 ? 8u * L.n_sm / ctas : 1;
+  if (c.D.align > 1 && c.T && ctas * slabs < ROWS_PAD_CTAS) ctas = (ROWS_PAD_CTAS + slabs - 1) / slabs;
+  return pm_launch(L, k_rows_dispatch_small<E, V>, dim3(ctas, slabs), 256, 0, c, ids, w, scale, (const E *)(c.T ? x : nullptr), (E *)rows);
 }
 
 cudaError_t launch_rows_dispatch(const Launch &L, const RowsCall &c, const uint32_t *ids, const float *w, bool scale, const void *x, void *rows) {

@@ -216,6 +216,9 @@ SHAPES = [
     dict(T=200, d=200, K=2, E=64, shift=1),                        # the buffer itself starts anywhere
     dict(T=500, d=24, K=4, E=32, first=8, local=8, none=0.2),      # a shard
     dict(T=400, d=40, K=4, E=33, first=32, local=1, align=16),     # a shard of one expert
+    dict(T=3, d=520, K=2, E=6, align=256),                         # a few pairs, nearly all rows are padding
+    dict(T=700, d=64, K=2, E=3, align=200),                        # ... of a few large groups
+    dict(T=100, d=49152, K=1, E=2),                                # the widest rows
     dict(T=2500, d=16, K=6, E=512, none=0.05),                     # more experts than most have pairs
 ]
 IDS = ["_".join(f"{k}{v}" for k, v in s.items()) for s in SHAPES]
