@@ -152,19 +152,10 @@ __global__ void __launch_bounds__(256) k_rows_dispatch_small(RowsCall c, const u
   __syncthreads();
   for (uint32_t v = v0; v < dv; v += gridDim.y * 256) {
     if (v != v0) mine = pm_load<E, V>(x + (size_t)t * c.D.x_stride + (size_t)v * V);
-    float f[V];
-    pm_widen<E, V>(mine, f);
-    for (int k = 0; k < K; k++) {
-      if (at[k] == PM_ROWS_NONE) continue;
-      Raw<E, V> o = mine;
-      if (scale) {
-        float g[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) g[i] = __fmul_rn(f[i], ws[k]);
-        o = pm_narrow<E, V>(g);
-      }
-      pm_store<E, V>(rows + (size_t)at[k] * c.D.rows_stride + (size_t)v * V, o);
-    }
+    const VecF<V> f = vf_widen<E, V>(mine);
+    for (int k = 0; k < K; k++)
+      if (at[k] != PM_ROWS_NONE)
+        pm_store<E, V>(rows + (size_t)at[k] * c.D.rows_stride + (size_t)v * V, scale ? vf_narrow<E, V>(vf_mul<V>(f, ws[k])) : mine);
   }
 }
 
@@ -278,17 +269,17 @@ __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS
 //   DOT      dw[t][k] = <rows[pos], src[t]>
 // G: a power of two, 256 at most (a CTA); grid.y cuts the rows of a few tokens without DOT further. Behind the tokens' CTAs
 // (SPREAD), some for each expert's padding. KB: K rounded up to one of five (10 pairs in a kernel for 16: 147 us instead of 126
-// for 8192 x 2048 bf16 with dot products). Rows that do not start on 16 bytes go value by value, two
-// values of a row a step and 32 warps an SM (8000 x 1001 f16 with dot products, 5 pairs: 74 us; one value a step 81, four values and 8 warps
-// 112), at about half of the speed of 16-byte words.
+// for 8192 x 2048 bf16 with dot products). Rows that do not start on 16 bytes go value by value, two values of a row a step and 32 warps an
+// SM (8000 x 1001 f16 with dot products, 5 pairs: 66 us, of 27 of bytes; four values a step and 8 warps 112).
 // CTAs that an SM is to hold: registers against reads in flight. Rows read as 16-byte words: 2 (8192 x 2048 bf16 with dot products 101 us; 1:
 // 130, 3: 104). Value by value: 4, of many pairs 2 (10 pairs: 4 spilled, 538 us against 363). Rows that are only written: any.
 __host__ __device__ constexpr int rows_ctas(int V, int KB, bool SPREAD, bool DOT) {
   return SPREAD && !DOT ? 1 : V == 1 && KB <= 8 ? 4 : 2;
 }
 template <typename E, int V, int KB, bool SPREAD, bool DOT>
-__global__ void __launch_bounds__(256, rows_ctas(V, KB, SPREAD, DOT)) k_rows(RowsCall c, uint32_t token_ctas, int G, const float *__restrict__ w, const E *__restrict__ src,
-                                              const E *__restrict__ rows, const E *add, E *out, float *__restrict__ dw) {
+__global__ void __launch_bounds__(256, rows_ctas(V, KB, SPREAD, DOT))
+    k_rows(RowsCall c, uint32_t token_ctas, int G, const float *__restrict__ w, const E *__restrict__ src, const E *__restrict__ rows, const E *add,
+           E *out, float *__restrict__ dw) {
   pm_pdl();
   __shared__ float sums[DOT ? 8 : 1][KB];
   const int tid = threadIdx.x;
@@ -314,7 +305,10 @@ __global__ void __launch_bounds__(256, rows_ctas(V, KB, SPREAD, DOT)) k_rows(Row
     dot[k] = 0;
   }
 #pragma unroll
-  for (int k = 0; k < KB; k++) pos[k] = rows_pos(c, pos[k]);
+  for (int k = 0; k < KB; k++) {
+    pos[k] = rows_pos(c, pos[k]);
+    if (pos[k] == PM_ROWS_NONE) wk[k] = 0.0f;  // (whatever its weight is, a NaN of a padded token's routing)
+  }
   // vectors of a step: single values come two at a time, so that their reads are in flight together
   constexpr int J = V > 1 ? 1 : 2;
   if (live)
@@ -361,6 +355,7 @@ __global__ void __launch_bounds__(256, rows_ctas(V, KB, SPREAD, DOT)) k_rows(Row
     for (int k = 0; k < KB; k++) {
       float a = vf_sum(dot[k]);
       for (int o = lanes / 2; o >= 1; o >>= 1) a = __fadd_rn(a, __shfl_xor_sync(PM_FULL, a, o));
+      if (pos[k] == PM_ROWS_NONE) a = 0.0f;  // (not 0 times an infinity of src)
       if (G <= 32) {
         if (live && tid % G == 0 && k < (int)K) dw[t * K + k] = a;
       } else if ((tid & 31) == 0) {

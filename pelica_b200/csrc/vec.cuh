@@ -6,10 +6,6 @@
 
 #include "common.cuh"
 
-template <typename E> struct VecOf {
-  static constexpr int N = 16 / sizeof(E);  // values of one 16-byte access
-};
-
 __device__ __forceinline__ float pm_to_f32(float v) { return v; }
 __device__ __forceinline__ float pm_to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float pm_to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -56,14 +52,6 @@ __device__ __forceinline__ void pm_narrow2(float *o, float a, float b) { o[0] = 
 __device__ __forceinline__ void pm_narrow2(__half *o, float a, float b) { *(__half2 *)o = __floats2half2_rn(a, b); }
 __device__ __forceinline__ void pm_narrow2(__nv_bfloat16 *o, float a, float b) { *(__nv_bfloat162 *)o = __floats2bfloat162_rn(a, b); }
 
-template <typename E, int V> __device__ __forceinline__ void pm_widen(const Raw<E, V> &r, float (&f)[V]) {
-  if constexpr (V == 1) {
-    f[0] = pm_to_f32(r.v[0]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i += 2) pm_unpack2(pm_widen2(&r.v[i]), f[i], f[i + 1]);
-  }
-}
 template <typename E, int V> __device__ __forceinline__ Raw<E, V> pm_narrow(const float (&f)[V]) {
   Raw<E, V> r;
   if constexpr (V == 1) {

@@ -301,6 +301,38 @@ def test_rows_without_values_stay_out_of_sums(tctx):
     assert bool(torch.isnan(y[0]).all()) and bool(torch.isfinite(y[2:]).all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d, pitch", [(40, 0), (40, 3), (2048, 0)])
+def test_padded_tokens_may_hold_anything(tctx, d, pitch, dtype):
+    """Routing weights that are NaN and values that are infinite in tokens without pairs stay where they are: sums over no row
+    are zeros (or add), the weights' gradients of pairs without a row are 0."""
+    c = Case(tctx, T=5, d=d, K=3, E=4, dtype=dtype, pitch=pitch, ids=torch.tensor([[0, 1, 2], [-1, -1, -1], [3, -1, 0], [-1, -1, -1], [2, 1, 3]]))
+    c.use_plan()
+    c.w[~c.has()] = float("nan")
+    c.w_d = c.w.cuda()
+    x, _ = c.stream(5)
+    x[1], x[3] = float("inf"), float("nan")
+    rows, _ = c.stream(c.max_rows)
+    y, _ = c.stream(5)
+    add, _ = c.stream(5)
+    dw = torch.full((5, 3), 55.0, device="cuda")
+    kw = dict(w=c.w_d.data_ptr())
+    c.op.collect(5, c.plan, rows.data_ptr(), y.data_ptr(), **kw)
+    tctx.sync()
+    assert bool(torch.isfinite(y).all()) and not y[1].any() and not y[3].any()
+    c.op.collect(5, c.plan, rows.data_ptr(), y.data_ptr(), add=add.data_ptr(), **kw)
+    tctx.sync()
+    assert torch.equal(y[1], add[1]) and torch.equal(y[3], add[3])
+    c.op.dispatch_grad(5, c.plan, rows.data_ptr(), y.data_ptr(), x=x.data_ptr(), dw=dw.data_ptr(), **kw)
+    tctx.sync()
+    assert bool(torch.isfinite(y).all()) and not y[1].any() and bool(torch.isfinite(dw).all()) and bool((dw.cpu()[~c.has()] == 0).all())
+    dw.fill_(55.0)
+    drows, _ = c.stream(c.max_rows, fill=False)
+    c.op.collect_grad(5, c.plan, x.data_ptr(), drows.data_ptr(), rows=rows.data_ptr(), dw=dw.data_ptr(), **kw)
+    tctx.sync()
+    assert bool(torch.isfinite(dw).all()) and bool((dw.cpu()[~c.has()] == 0).all()) and bool(torch.isfinite(drows[:c.total]).all())
+
+
 @pytest.mark.parametrize("T", [5, 600])
 def test_ids_that_no_expert_has_are_left_out_and_reported(tctx, T):
     c = Case(tctx, T=T, d=32, K=3, E=7, align=4)
