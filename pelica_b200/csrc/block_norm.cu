@@ -20,8 +20,14 @@ namespace cg = cooperative_groups;
 // the registers of an SM do not hold), a CTA has rpb groups, each with rows of its own. Rows of a group follow one another; a
 // thread copies its own values of the next ones into its own slots of shared memory (cp.async) while it works on one, so that
 // the bytes in flight do not depend on registers and no thread waits for another's copy.
-#define NORM_FWD_VALUES 8192   // values of rows resident on an SM
-#define NORM_GRAD_VALUES(n) ((n) == 16 ? 8192 : 7168)  // ... backward, with n values a thread: 512 threads of 128 registers, 896 of 72
+// Values of rows that an SM holds, in whole CTAs: forward 16 values a thread in 896 threads (two rows of 7,168 values: 4096 x 7168 bf16 41 us, one
+// row at a time 58), in 1,024 for wider rows (4096 x 8192 51 us, with 896 62; 4096 x 7168 47), 8 values in 1,024; backward, whose column sums
+// take registers, 16 values in 512, 8 in 896.
+#define NORM_FWD 14336
+#define NORM_FWD_WIDE 16384
+#define NORM_FWD_8 8192
+#define NORM_GRAD 8192
+#define NORM_GRAD_8 7168
 #define NORM_SMEM 233472      // bytes of shared memory of an SM, of which every CTA takes
 #define NORM_SMEM_CTA 2560    // ... these for its sums and for itself
 struct NormShape {
@@ -246,8 +252,9 @@ template <typename W> __device__ __forceinline__ float norm_token_gate(const Nor
 //   NORM_BEFORE    the norm before the next block only, every stream
 enum NormMode { NORM_ANY, NORM_SANDWICH, NORM_BEFORE };
 
-template <typename E, typename W, int V, int N, bool CLUSTER, bool RING, NormMode MODE>
-__global__ void __launch_bounds__(NORM_FWD_VALUES / N) k_block_norm(NormCall c, int tpr, int rpb, int cl, int stages) {
+// SM: values of rows that an SM holds
+template <typename E, typename W, int V, int N, int SM, bool CLUSTER, bool RING, NormMode MODE>
+__global__ void __launch_bounds__(SM / N) k_block_norm(NormCall c, int tpr, int rpb, int cl, int stages) {
   pm_pdl();
   extern __shared__ uint4 slots[];
   __shared__ NormRed<1> red;
@@ -258,7 +265,7 @@ __global__ void __launch_bounds__(NORM_FWD_VALUES / N) k_block_norm(NormCall c, 
   const bool post = ANY ? c.D.flags & PM_NORM_POST : MODE == NORM_SANDWICH, pre = ANY ? c.D.flags & PM_NORM_PRE : true;
   const bool has_x = ANY ? c.x != nullptr : true, has_f = ANY ? c.f != nullptr : true, has_r = ANY ? c.r != nullptr : true;
   const int i_x = has_f ? 1 : 0;
-  const NormRing<E, V, N, RING> ring = {norm_slots(slots), 0, i_x + (has_x ? 1 : 0), stages};
+  const NormRing<E, V, N, RING> ring = {norm_slots(slots), N / 2, i_x + (has_x ? 1 : 0), stages};
   const int t0 = (int)(blockIdx.x / at.cl) * rpb + at.group;
   auto copy = [&](int stage, int t) {
     if (t < c.T) {
@@ -272,8 +279,12 @@ __global__ void __launch_bounds__(NORM_FWD_VALUES / N) k_block_norm(NormCall c, 
   if constexpr (RING)
     for (int s = 0; s < stages; s++) copy(s, t0 + s * groups);
   VecF<N> wp = norm_weights<W, V, N>(post ? c.w_post : nullptr, c.D.offset_post, at, d);  // gate and post weight
-  const VecF<N> wn = norm_weights<W, V, N>(pre ? c.w_pre : nullptr, c.D.offset_pre, at, d);
+  VecF<N> wn = norm_weights<W, V, N>(pre ? c.w_pre : nullptr, c.D.offset_pre, at, d);
   if (c.D.gate == PM_NORM_GATE_CHANNEL) wp = wp * norm_weights<W, V, N>(c.gate, 0.0f, at, d);
+  if constexpr (RING) {  // (read again for each row: the registers are the rows')
+    ring.slots.template put_vec<N>(0, wp);
+    ring.slots.template put_vec<N>(N / 4, wn);
+  }
   int turn = 0, stage = 0;
   for (int t = t0; t < c.T; t += groups) {
     NormRow<E, V, N> xr, fr;
@@ -285,6 +296,7 @@ __global__ void __launch_bounds__(NORM_FWD_VALUES / N) k_block_norm(NormCall c, 
       copy(stage, t + stages * groups);
       stage = stage + 1 == stages ? 0 : stage + 1;
     }
+    if constexpr (RING) wp = ring.slots.template get_vec<N>(0);
     VecF<N> r = has_x ? xr.widen() * c.D.alpha : vf_all<N>(0.0f);
     if (has_f) {
       const VecF<N> f = fr.widen();
@@ -300,6 +312,7 @@ __global__ void __launch_bounds__(NORM_FWD_VALUES / N) k_block_norm(NormCall c, 
     if (pre) {
       float sum[1] = {vf_dot(r, r)};
       norm_sum<1, CLUSTER>(sum, at, red, peer, turn);
+      if constexpr (RING) wn = ring.slots.template get_vec<N>(N / 4);
       NormRow<E, V, N>::store(c.n, norm_row(t, c.D.n_stride), at, d, r * wn * norm_inv(sum[0], c.inv_d, c.D.eps_pre));
     }
   }
@@ -310,8 +323,8 @@ __global__ void __launch_bounds__(NORM_FWD_VALUES / N) k_block_norm(NormCall c, 
 // are read again from the ring each time and the weights lie beside it (f32, the thread's own columns): the 16 sums of the
 // weights' gradients fill the registers. A CTA adds up its groups and leaves a row of sums in parts[kind][CTA][d], which
 // k_norm_sum_parts adds up. No atomics.
-template <typename E, typename W, int V, int N, bool CLUSTER, bool RING, NormMode MODE>
-__global__ void __launch_bounds__(NORM_GRAD_VALUES(N) / N) k_block_norm_grad(NormCall c, int tpr, int rpb, int cl, int stages) {
+template <typename E, typename W, int V, int N, int SM, bool CLUSTER, bool RING, NormMode MODE>
+__global__ void __launch_bounds__(SM / N) k_block_norm_grad(NormCall c, int tpr, int rpb, int cl, int stages) {
   pm_pdl();
   extern __shared__ uint4 slots[];
   __shared__ NormRed<3> red3;
@@ -471,23 +484,20 @@ static int norm_parts(const NormShape &s, int T, int n_sm) {
   const int need = (T + s.rpb - 1) / s.rpb;
   return need < most ? need : most;
 }
-// Values a thread holds where rows are whole 16-byte words. Backward: 16 of the 16-bit types, half the threads for the same sums (4096 x 2048 bf16
-// 31 -> 28 us, x 4096 60 -> 56, x 7168 even), 8 of f32, whose rings are twice the size (4096 x 7168: 145 us, 159 with 16). Forward:
-// 16 for rows of up to 2,048 16-bit values (16384 x 512: 11.6 -> 9.9 us, x 2048 52.4 -> 50.9; 8192 x 4096: 55.5 -> 58.0).
-static int norm_values(const pm_norm_desc &D, bool grad) { return D.dtype != PM_TYPE_F32 && (grad || D.d <= 2048) ? 16 : 8; }
 size_t norm_parts_floats(const pm_norm_desc &D, int T, int n_sm) {
   size_t most = 0;  // (of both forms of a row: which one is taken goes by the buffers)
-  for (int n : {8, norm_values(D, true)}) {
-    const size_t f = (size_t)3 * norm_parts(norm_shape(D.d, n, NORM_GRAD_VALUES(n)), T, n_sm) * D.d;
+  for (int n : {8, 16}) {
+    const size_t f = (size_t)3 * norm_parts(norm_shape(D.d, n, n == 16 ? NORM_GRAD : NORM_GRAD_8), T, n_sm) * D.d;
     if (f > most) most = f;
   }
   return most;
 }
 
-// the rows of `row` slots that fit into a ring beside `fixed` slots a thread, 3 at most; fewer CTAs on an SM where two would not fit
+// the rows of `row` slots that fit into a ring beside `fixed` slots a thread, 3 at most; fewer CTAs on an SM where not one would fit
+// (two CTAs with a row ahead each are better than one with three: forward 4096 x 7168 41 us, 58)
 static void norm_ring(NormShape &s, int fixed, int row) {
   auto fit = [&](int per_sm) { return ((NORM_SMEM / per_sm - NORM_SMEM_CTA) / (s.threads() * 16) - fixed) / row; };
-  while (s.per_sm > 1 && fit(s.per_sm) < 2) s.per_sm--;
+  while (s.per_sm > 1 && fit(s.per_sm) < 1) s.per_sm--;
   const int n = fit(s.per_sm);
   s.stages = n > 3 ? 3 : n < 1 ? 1 : n;
   s.slots = fixed + s.stages * row;
@@ -514,60 +524,62 @@ static cudaError_t norm_launch(const Launch &L, SmemOptIn &opt, void (*kern)(P..
   if (L.count) ++*L.count;
   return cudaLaunchKernelEx(&cfg, kern, c, s.tpr, s.rpb, s.cl, s.stages);
 }
-template <typename E, typename W, int V, int N, bool RING, NormMode MODE, bool GRAD>
+template <typename E, typename W, int V, int N, int SM, bool RING, NormMode MODE, bool GRAD>
 static cudaError_t norm_go(const Launch &L, int parts, const NormShape &s, const NormCall &c) {
   static SmemOptIn one, many;
   if constexpr (GRAD)
-    return s.cl > 1 ? norm_launch(L, many, k_block_norm_grad<E, W, V, N, true, RING, MODE>, parts, s, c)
-                    : norm_launch(L, one, k_block_norm_grad<E, W, V, N, false, RING, MODE>, parts, s, c);
+    return s.cl > 1 ? norm_launch(L, many, k_block_norm_grad<E, W, V, N, SM, true, RING, MODE>, parts, s, c)
+                    : norm_launch(L, one, k_block_norm_grad<E, W, V, N, SM, false, RING, MODE>, parts, s, c);
   else
-    return s.cl > 1 ? norm_launch(L, many, k_block_norm<E, W, V, N, true, RING, MODE>, parts, s, c)
-                    : norm_launch(L, one, k_block_norm<E, W, V, N, false, RING, MODE>, parts, s, c);
+    return s.cl > 1 ? norm_launch(L, many, k_block_norm<E, W, V, N, SM, true, RING, MODE>, parts, s, c)
+                    : norm_launch(L, one, k_block_norm<E, W, V, N, SM, false, RING, MODE>, parts, s, c);
 }
 // the kernels of 16-byte words that go by what the call has
-template <typename E, typename W, int V, int N, bool GRAD>
+template <typename E, typename W, int V, int N, int SM, bool GRAD>
 static cudaError_t norm_go_mode(const Launch &L, int parts, const NormShape &s, const NormCall &c) {
   const bool all = GRAD ? c.dr && c.dx && c.df : c.x && c.f && c.r;
   const bool post = c.D.flags & PM_NORM_POST, pre = c.D.flags & PM_NORM_PRE;
-  if (all && pre && post) return norm_go<E, W, V, N, true, NORM_SANDWICH, GRAD>(L, parts, s, c);
-  if (all && pre && c.D.gate == PM_NORM_GATE_NONE) return norm_go<E, W, V, N, true, NORM_BEFORE, GRAD>(L, parts, s, c);
-  return norm_go<E, W, V, N, true, NORM_ANY, GRAD>(L, parts, s, c);
+  if (all && pre && post) return norm_go<E, W, V, N, SM, true, NORM_SANDWICH, GRAD>(L, parts, s, c);
+  if (all && pre && c.D.gate == PM_NORM_GATE_NONE) return norm_go<E, W, V, N, SM, true, NORM_BEFORE, GRAD>(L, parts, s, c);
+  return norm_go<E, W, V, N, SM, true, NORM_ANY, GRAD>(L, parts, s, c);
 }
 
 // rows of 16-byte words, more of them than groups: through rings
-template <typename E, typename W, int V, int N> static cudaError_t norm_forward_ring(const Launch &L, const NormCall &c) {
-  NormShape s = norm_shape(c.D.d, N, NORM_FWD_VALUES);
-  norm_ring(s, 0, ((c.x ? 1 : 0) + (c.f ? 1 : 0)) * N / V);
-  return norm_go_mode<E, W, V, N, false>(L, norm_parts(s, c.T, L.n_sm), s, c);
+template <typename E, typename W, int V, int N, int SM> static cudaError_t norm_forward_ring(const Launch &L, const NormCall &c) {
+  NormShape s = norm_shape(c.D.d, N, SM);
+  norm_ring(s, N / 2, ((c.x ? 1 : 0) + (c.f ? 1 : 0)) * N / V);
+  return norm_go_mode<E, W, V, N, SM, false>(L, norm_parts(s, c.T, L.n_sm), s, c);
 }
+// 16 values a thread of the 16-bit types, half the threads for the same sums (gradient of 4096 x 2048 bf16 31 -> 28 us, x 4096 60 -> 56); 8 of
+// f32, whose rings are twice the size (gradient of 4096 x 7168: 145 us, 159 with 16), of rows value by value, and of a row a group (no ring).
 template <typename E, typename W, int V> static cudaError_t norm_forward(const Launch &L, const NormCall &c) {
-  const NormShape s = norm_shape(c.D.d, 8, NORM_FWD_VALUES);
+  const NormShape s = norm_shape(c.D.d, 8, NORM_FWD_8);
   const int parts = norm_parts(s, c.T, L.n_sm);
   if constexpr (V > 1) {
     if (c.T > parts * s.rpb) {
-      if constexpr (V == 8) if (norm_values(c.D, false) == 16) return norm_forward_ring<E, W, V, 16>(L, c);
-      return norm_forward_ring<E, W, V, 8>(L, c);
+      if constexpr (V == 4) return norm_forward_ring<E, W, V, 8, NORM_FWD_8>(L, c);
+      else if (c.D.d > NORM_FWD / 2) return norm_forward_ring<E, W, V, 16, NORM_FWD_WIDE>(L, c);
+      else return norm_forward_ring<E, W, V, 16, NORM_FWD>(L, c);
     }
   }
-  return norm_go<E, W, V, 8, false, NORM_ANY, false>(L, parts, s, c);
+  return norm_go<E, W, V, 8, NORM_FWD_8, false, NORM_ANY, false>(L, parts, s, c);
 }
-template <typename E, typename W, int V, int N> static cudaError_t norm_backward_rows(const Launch &L, const NormCall &c, int *parts) {
-  NormShape s = norm_shape(c.D.d, N, NORM_GRAD_VALUES(N));
+template <typename E, typename W, int V> static cudaError_t norm_backward_rows(const Launch &L, const NormCall &c, int *parts) {
+  constexpr int N = V == 8 ? 16 : 8, SM = V == 8 ? NORM_GRAD : NORM_GRAD_8;
+  NormShape s = norm_shape(c.D.d, N, SM);
   const bool post = c.D.flags & PM_NORM_POST, pre = c.D.flags & PM_NORM_PRE, gate = c.D.gate != PM_NORM_GATE_NONE;
   const int row = ((pre ? 2 : 0) + (post || gate ? 1 : 0) + (c.dr ? 1 : 0)) * N / V;
   s.slots = N / 2;
   if (V > 1 && row) norm_ring(s, N / 2, row);
   *parts = norm_parts(s, c.T, L.n_sm);
-  if constexpr (V > 1) return norm_go_mode<E, W, V, N, true>(L, *parts, s, c);
-  else return norm_go<E, W, V, N, false, NORM_ANY, true>(L, *parts, s, c);
+  if constexpr (V > 1) return norm_go_mode<E, W, V, N, SM, true>(L, *parts, s, c);
+  else return norm_go<E, W, V, N, SM, false, NORM_ANY, true>(L, *parts, s, c);
 }
 template <typename E, typename W, int V> static cudaError_t norm_backward(const Launch &L, const NormCall &c) {
   int parts = 0;
   float *channel = c.D.gate == PM_NORM_GATE_CHANNEL ? c.dgate : nullptr;
   if (c.T) {  // (no rows: the sums alone, zeros)
-    cudaError_t e;
-    if constexpr (V == 8) e = norm_backward_rows<E, W, V, 16>(L, c, &parts);  // (norm_values)
-    else e = norm_backward_rows<E, W, V, 8>(L, c, &parts);
+    const cudaError_t e = norm_backward_rows<E, W, V>(L, c, &parts);
     if (e != cudaSuccess) return e;
   }
   if (!c.dw_pre && !c.dw_post && !channel) return cudaSuccess;
