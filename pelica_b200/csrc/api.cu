@@ -2259,17 +2259,28 @@ extern "C" int32_t pm_stack_set_norm(pm_stack *s, int32_t layer, const pm_norm_d
       *to[i] = p;
     }
   }
-  CU(cudaStreamSynchronize(s->ctx->stream));  // nothing uses what is replaced, and the copies are done
+  const cudaError_t done = cudaStreamSynchronize(s->ctx->stream);  // nothing uses what is replaced, and the copies are done
+  if (done != cudaSuccess) {
+    cudaGetLastError();
+    cudaFree(n.buf);
+    return fail(PM_ERR_CUDA, "%s: %s", call, cudaGetErrorString(done));
+  }
   if (s->norms.empty()) {
     if (!norm) return PM_OK;
-    s->norms.assign(L, stack_plain_norm(s));
+    try {
+      s->norms.assign(L, stack_plain_norm(s));
+    } catch (const std::bad_alloc &) {
+      cudaFree(n.buf);
+      return fail(PM_ERR_OOM, "%s: host allocation", call);
+    }
   }
   stack_drop_graphs(s);
-  if (s->norms[layer].buf) CU(cudaFree(s->norms[layer].buf));
+  float *old = s->norms[layer].buf;
   s->norms[layer] = n;
   bool any = false;
   for (const pm_stack::Norm &q : s->norms) any = any || q.buf;
   if (!any) s->norms.clear();
+  CU(cudaFree(old));
   return PM_OK;
 }
 

@@ -240,7 +240,8 @@ def test_all_calls(tctx, shape, dtype):
     run_collect_grad(c, weighted=False, dw=True)
 
 
-@pytest.mark.parametrize("T, K, E, align", [(16384, 16, 512, 1), (16384, 8, 3, 16), (4097, 7, 200, 5), (16384, 1, 512, 256)])
+@pytest.mark.parametrize("T, K, E, align", [(16384, 16, 512, 1), (16384, 8, 3, 16), (4097, 7, 200, 5), (16384, 1, 512, 256),
+                                            (1024, 4, 64, 1), (4100, 1, 9, 4), (8192, 1, 77, 1), (8193, 1, 77, 2), (8193, 8, 300, 1)])
 def test_large_sorts(tctx, T, K, E, align):
     c = Case(tctx, T=T, d=8, K=K, E=E, align=align, none=0.02, seed=T + K)
     run_dispatch(c, scale=False)
