@@ -29,7 +29,7 @@ namespace cg = cooperative_groups;
 #define NORM_GRAD 8192
 #define NORM_GRAD_8 7168
 #define NORM_SMEM 233472      // bytes of shared memory of an SM, of which every CTA takes
-#define NORM_SMEM_CTA 2560    // ... these for its sums and for itself
+#define NORM_SMEM_CTA 3584    // ... these for its sums and for itself
 struct NormShape {
   int tpr, rpb, cl;   // threads of a row's group in a CTA, groups of a CTA, CTAs of a row
   int stages;         // rows in a group's ring, 0: none
@@ -53,28 +53,34 @@ struct NormPlace {
   int lane, warp, group, tpr, cl, rank, col0;
 };
 
-// sums over a warp: of one value, in every lane; of three, value q in the lanes with lane & 3 == q
+// sums over a warp: of one value, in every lane; of up to eight, value q in the lanes with lane & 7 == q
 template <int N> __device__ __forceinline__ float norm_warp_sums(const float (&v)[N], int lane) {
-  static_assert(N == 1 || N == 3, "");
+  static_assert(N <= 6, "");
   if constexpr (N == 1) return pm_warp_sum_16_1(v[0]);
-  else {  // lanes of a quad keep one value each: 2 + 1 + 3 exchanges for 15
-    const bool b0 = lane & 1, b1 = lane & 2;
-    const float a = __fadd_rn(b0 ? v[1] : v[0], __shfl_xor_sync(PM_FULL, b0 ? v[0] : v[1], 1));  // values 0, 1
-    const float c = __fadd_rn(b0 ? 0.0f : v[2], __shfl_xor_sync(PM_FULL, b0 ? v[2] : 0.0f, 1));  // value 2
-    float s = __fadd_rn(b1 ? c : a, __shfl_xor_sync(PM_FULL, b1 ? a : c, 2));
+  else {  // lanes of eight keep one value each: 3 + 2 + 1 + 2 exchanges for 30
+    const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
+    float a[3], b[2];
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) s = __fadd_rn(s, __shfl_xor_sync(PM_FULL, s, o));
+    for (int j = 0; j < 3; j++) {
+      const float e = 2 * j < N ? v[2 * j < N ? 2 * j : 0] : 0.0f, o = 2 * j + 1 < N ? v[2 * j + 1 < N ? 2 * j + 1 : 0] : 0.0f;
+      a[j] = 2 * j < N ? __fadd_rn(b0 ? o : e, __shfl_xor_sync(PM_FULL, b0 ? e : o, 1)) : 0.0f;
+    }
+    b[0] = __fadd_rn(b1 ? a[1] : a[0], __shfl_xor_sync(PM_FULL, b1 ? a[0] : a[1], 2));
+    b[1] = N > 4 ? __fadd_rn(b1 ? 0.0f : a[2], __shfl_xor_sync(PM_FULL, b1 ? a[2] : 0.0f, 2)) : 0.0f;
+    float s = __fadd_rn(b2 ? b[1] : b[0], __shfl_xor_sync(PM_FULL, b2 ? b[0] : b[1], 4));
+#pragma unroll
+    for (int o = 8; o < 32; o <<= 1) s = __fadd_rn(s, __shfl_xor_sync(PM_FULL, s, o));
     return s;
   }
 }
 
 // Sums of N values over a row's group, in every thread: lanes, then warps through red (two turns used alternately, so that one
 // barrier a sum is enough), then the cluster's CTAs.
-template <int N> using NormRed = float[2][N == 1 ? 1 : 4][32];
+template <int N> using NormRed = float[2][N == 1 ? 1 : 8][32];
 template <int N> using NormPeer = float[2][8][N];
 template <int N, bool CLUSTER>
 __device__ __forceinline__ void norm_sum(float (&v)[N], const NormPlace &at, NormRed<N> &red, NormPeer<N> &peer, int &turn) {
-  constexpr int Q = N == 1 ? 1 : 4;
+  constexpr int Q = N == 1 ? 1 : 8;
   float s = norm_warp_sums<N>(v, at.lane);
   const int warps = at.tpr >> 5;
   if (warps > 1 || CLUSTER) {
@@ -88,9 +94,9 @@ __device__ __forceinline__ void norm_sum(float (&v)[N], const NormPlace &at, Nor
   }
   if constexpr (CLUSTER) {
     cg::cluster_group cluster = cg::this_cluster();
-    // lane i * Q + q of the first warp gives sum q to CTA i
-    if (at.warp == 0 && at.lane < at.cl * Q && (at.lane & (Q - 1)) < N)
-      cluster.map_shared_rank(&peer[turn][at.rank][0], at.lane / Q)[at.lane & (Q - 1)] = s;
+    // the first warp's lanes give sum i % Q to CTA i / Q
+    if (at.warp == 0 && (at.lane & (Q - 1)) < N)
+      for (int i = at.lane; i < at.cl * Q; i += 32) cluster.map_shared_rank(&peer[turn][at.rank][0], i / Q)[i & (Q - 1)] = s;
     cluster.sync();
 #pragma unroll
     for (int i = 0; i < N; i++) {
@@ -319,18 +325,18 @@ __global__ void __launch_bounds__(SM / N) k_block_norm(NormCall c, int tpr, int 
   if constexpr (CLUSTER) cg::this_cluster().sync();  // no CTA leaves while another may still write its sums here
 }
 
-// Three sweeps over a row's values: the sums of both norms; D, dx, the weights' gradients and the sum of v f; df. The values
-// are read again from the ring each time and the weights lie beside it (f32, the thread's own columns): the 16 sums of the
-// weights' gradients fill the registers. A CTA adds up its groups and leaves a row of sums in parts[kind][CTA][d], which
-// k_norm_sum_parts adds up. No atomics.
+// Two sweeps over a row's values. The first makes all sums that the row needs at once: with q = g f (o1 + w_post), the sum of v f is linear
+// in D, so <D, q> = <dr, q> + s2 (<u, q> - s2^2 mean(u r) <r, q>) needs no D, and one exchange between the warps does where
+// two lay on the chain. The second sweep makes dx, df and the weights' gradients. The values are read from the ring each time and
+// the weights lie beside it (f32, the thread's own columns): the sums of the weights' gradients fill the registers. A CTA adds up
+// its groups and leaves a row of sums in parts[kind][CTA][d], which k_norm_sum_parts adds up. No atomics.
 template <typename E, typename W, int V, int N, int SM, bool CLUSTER, bool RING, NormMode MODE>
 __global__ void __launch_bounds__(SM / N) k_block_norm_grad(NormCall c, int tpr, int rpb, int cl, int stages) {
   pm_pdl();
   extern __shared__ uint4 slots[];
-  __shared__ NormRed<3> red3;
-  __shared__ NormPeer<3> peer3;
-  __shared__ NormRed<1> red;
-  __shared__ NormPeer<1> peer;
+  constexpr int SUMS = MODE == NORM_BEFORE ? 2 : 6;  // r r, u r; f f, dr q, u q, r q
+  __shared__ NormRed<SUMS> red;
+  __shared__ NormPeer<SUMS> peer;
   const NormPlace at = norm_place<CLUSTER>(tpr, cl, V);
   const int d = c.D.d, n_parts = (int)(gridDim.x / at.cl), part = (int)(blockIdx.x / at.cl), groups = n_parts * rpb;
   constexpr bool ANY = MODE == NORM_ANY;
@@ -361,34 +367,48 @@ __global__ void __launch_bounds__(SM / N) k_block_norm_grad(NormCall c, int tpr,
   own.template put_vec<N>(0, norm_weights<W, V, N>(pre ? c.w_pre : nullptr, c.D.offset_pre, at, d));
   own.template put_vec<N>(N / 4, norm_weights<W, V, N>(post ? c.w_post : nullptr, c.D.offset_post, at, d) * norm_weights<W, V, N>(channel ? c.gate : nullptr, 0.0f, at, d));
   VecF<N> a_pre = vf_all<N>(0.0f), a_dk = vf_all<N>(0.0f);
-  int turn3 = 0, turn = 0, stage = 0;
+  int turn = 0, stage = 0;
   for (int t = t0; t < c.T; t += groups) {
     const size_t at_r = norm_row(t, c.D.r_stride), at_f = norm_row(t, c.D.f_stride), at_n = norm_row(t, c.D.n_stride);
     const uint32_t row = ring.row(stage);
-    NormRow<E, V, N> raw, fr;
-    float sum[3] = {0.0f, 0.0f, 0.0f};
+    NormRow<E, V, N> raw;
+    float sum[SUMS] = {};
     ring.wait();
-    if (pre) {
-      ring.get(raw, row, 0, c.x, at_r, at, d);
-      const VecF<N> r = raw.widen();
-      ring.get(raw, row, 1, c.dn, at_n, at, d);
-      sum[0] = vf_dot(r, r);
-      sum[1] = vf_dot(raw.widen() * own.template get_vec<N>(0), r);
+    {
+      VecF<N> q;
+      if (use_f) {
+        ring.get(raw, row, i_f, c.f, at_f, at, d);
+        q = raw.widen();
+        if (post) sum[SUMS > 2 ? 2 : 0] = vf_dot(q, q);
+        q = q * own.template get_vec<N>(N / 4);
+        if (has_dr) {
+          ring.get(raw, row, i_dr, c.dr, at_r, at, d);
+          sum[SUMS > 2 ? 3 : 0] = vf_dot(raw.widen(), q);
+        }
+      }
+      if (pre) {
+        ring.get(raw, row, 0, c.x, at_r, at, d);
+        const VecF<N> r = raw.widen();
+        ring.get(raw, row, 1, c.dn, at_n, at, d);
+        const VecF<N> u = raw.widen() * own.template get_vec<N>(0);
+        sum[0] = vf_dot(r, r);
+        sum[1] = vf_dot(u, r);
+        if (use_f) {
+          sum[SUMS > 2 ? 4 : 0] = vf_dot(u, q);
+          sum[SUMS > 2 ? 5 : 0] = vf_dot(r, q);
+        }
+      }
     }
-    if (use_f) ring.get(fr, row, i_f, c.f, at_f, at, d);
-    if (post) {
-      const VecF<N> f = fr.widen();
-      sum[2] = vf_dot(f, f);
-    }
-    if (pre || post) norm_sum<3, CLUSTER>(sum, at, red3, peer3, turn3);
+    if (pre || post || token) norm_sum<SUMS, CLUSTER>(sum, at, red, peer, turn);
     VecF<N> D = vf_all<N>(0.0f);
     if (has_dr) {
       ring.get(raw, row, i_dr, c.dr, at_r, at, d);
       D = raw.widen();
     }
+    float s2 = 0.0f, m = 0.0f;
     if (pre) {
-      const float s2 = norm_inv(sum[0], c.inv_d, c.D.eps_pre);
-      const float m = __fmul_rn(__fmul_rn(s2, s2), __fmul_rn(sum[1], c.inv_d));
+      s2 = norm_inv(sum[0], c.inv_d, c.D.eps_pre);
+      m = __fmul_rn(__fmul_rn(s2, s2), __fmul_rn(sum[1], c.inv_d));
       ring.get(raw, row, 0, c.x, at_r, at, d);
       const VecF<N> r = raw.widen();
       ring.get(raw, row, 1, c.dn, at_n, at, d);
@@ -396,35 +416,27 @@ __global__ void __launch_bounds__(SM / N) k_block_norm_grad(NormCall c, int tpr,
       a_pre = vf_fma(dn, r * s2, a_pre);
       D = vf_fma(vf_fma(r, -m, dn * own.template get_vec<N>(0)), s2, D);
     }
-    if constexpr (RING) {  // (f is in registers)
+    if (has_dx) NormRow<E, V, N>::store(c.dx, norm_row(t, c.D.x_stride), at, d, D * c.D.alpha);
+    // k = f s1; D becomes beta g D (o1 + w_post); gt: the token's gate
+    const float gt = MODE == NORM_BEFORE ? 1.0f : norm_token_gate<W>(c, t);
+    D = D * __fmul_rn(c.D.beta, gt);
+    if constexpr (SUMS > 2) {
+      if (use_f) {
+        const float s1 = post ? norm_inv(sum[2], c.inv_d, c.D.eps_post) : 1.0f;
+        const float dot = __fmul_rn(__fmul_rn(c.D.beta, s1), __fmaf_rn(s2, __fmaf_rn(-m, sum[5], sum[4]), sum[3]));
+        if (token && c.dgate && at.rank == 0 && at.warp == 0 && at.lane == 0) c.dgate[t] = dot;
+        ring.get(raw, row, i_f, c.f, at_f, at, d);
+        const VecF<N> k = raw.widen() * s1;
+        if (post || channel) a_dk = vf_fma(D, k, a_dk);
+        D = D * own.template get_vec<N>(N / 4);
+        if (post) D = vf_fma(k, -__fmul_rn(__fmul_rn(dot, gt), c.inv_d), D) * s1;
+      }
+    }
+    if constexpr (RING) {
       copy(stage, t + stages * groups);
       stage = stage + 1 == stages ? 0 : stage + 1;
     }
-    if (has_dx) NormRow<E, V, N>::store(c.dx, norm_row(t, c.D.x_stride), at, d, D * c.D.alpha);
-    if (!use_f && !has_df) continue;
-    // D becomes beta g D, g of the token, then beta g D (o1 + w_post) of either gate; k = f s1
-    const float gt = MODE == NORM_BEFORE ? 1.0f : norm_token_gate<W>(c, t);
-    float s1 = 1.0f, mean = 0.0f;
-    if (use_f) {
-      if (post) s1 = norm_inv(sum[2], c.inv_d, c.D.eps_post);
-      const VecF<N> k = fr.widen() * s1;
-      D = D * c.D.beta;
-      if (post || channel) a_dk = vf_fma(D * gt, k, a_dk);
-      D = D * own.template get_vec<N>(N / 4);
-      if (post || token) {
-        float dot[1] = {vf_dot(D, k)};
-        norm_sum<1, CLUSTER>(dot, at, red, peer, turn);
-        if (token && c.dgate && at.rank == 0 && at.warp == 0 && at.lane == 0) c.dgate[t] = dot[0];
-        mean = __fmul_rn(__fmul_rn(dot[0], gt), c.inv_d);
-      }
-      D = D * gt;
-    } else {
-      D = D * c.D.beta;
-    }
-    if (has_df) {
-      if (post) D = vf_fma(fr.widen() * s1, -mean, D) * s1;
-      NormRow<E, V, N>::store(c.df, at_f, at, d, D);
-    }
+    if (has_df) NormRow<E, V, N>::store(c.df, at_f, at, d, D);
   }
   // The CTA's groups, kind by kind, columns of a thread as it holds them. With K = sum over t of beta g_t D k, dw_post is K times
   // the channel's gate and the channel's dgate is K times the post weight.
