@@ -543,7 +543,7 @@ NORM_GATES = {"none": 0, "channel": 1, "token": 2}
 
 def _dev(p):
     """A device pointer: an address, a DevBuf, or anything with its address in `ptr`; None stays None."""
-    return p if p is None or isinstance(p, int) else p.ptr
+    return p if p is None or p.__class__ is int else p.ptr
 
 
 class Rows:
@@ -554,11 +554,12 @@ class Rows:
                  align: int = 1, x_stride: int = 0, rows_stride: int = 0):
         self.ctx, self.lib = ctx, ctx.lib
         self.desc = RowsDesc(STREAM_TYPES[dtype], d, top_k, n_exp, first_expert, n_local, align, 0, x_stride, rows_stride)
+        self._desc = C.byref(self.desc)
         self.bound(0)
 
     def bound(self, T: int) -> int:
         """Rows that T tokens can need, the padding of the groups included."""
-        n = self.lib.pm_rows_bound(C.byref(self.desc), T)
+        n = self.lib.pm_rows_bound(self._desc, T)
         if n < 0:
             _check(n)
         return n
@@ -570,21 +571,27 @@ class Rows:
     def dispatch(self, T: int, ids, plan: RowsPlan, x=None, rows=None, w=None, scale: bool = True):
         """Fills the plan from ids [T, top_k]; rows[pos] = x[t], times w with `scale` and w given."""
         flags = PM_ROWS_SCALE if scale and w is not None else 0
-        _check(self.lib.pm_dispatch_rows(self.ctx.h, C.byref(self.desc), T, _dev(ids), _dev(w), C.byref(plan), _dev(x), _dev(rows), flags))
+        rc = self.lib.pm_dispatch_rows(self.ctx.h, self._desc, T, _dev(ids), _dev(w), plan, _dev(x), _dev(rows), flags)
+        if rc:
+            _check(rc)
 
     def dispatch_grad(self, T: int, plan: RowsPlan, drows, dx, w=None, x=None, dw=None):
         """dx[t] = sum_k w drows[pos]; dw = <drows[pos], x[t]>."""
-        _check(self.lib.pm_dispatch_rows_grad(self.ctx.h, C.byref(self.desc), T, C.byref(plan), _dev(w), _dev(x), _dev(drows), _dev(dx),
-                                              _dev(dw)))
+        rc = self.lib.pm_dispatch_rows_grad(self.ctx.h, self._desc, T, plan, _dev(w), _dev(x), _dev(drows), _dev(dx), _dev(dw))
+        if rc:
+            _check(rc)
 
     def collect(self, T: int, plan: RowsPlan, rows, y, w=None, add=None):
         """y[t] = add[t] + sum_k w rows[pos]."""
-        _check(self.lib.pm_collect_rows(self.ctx.h, C.byref(self.desc), T, C.byref(plan), _dev(w), _dev(rows), _dev(add), _dev(y)))
+        rc = self.lib.pm_collect_rows(self.ctx.h, self._desc, T, plan, _dev(w), _dev(rows), _dev(add), _dev(y))
+        if rc:
+            _check(rc)
 
     def collect_grad(self, T: int, plan: RowsPlan, dy, drows, w=None, rows=None, dw=None):
         """drows[pos] = w dy[t]; dw = <rows[pos], dy[t]>."""
-        _check(self.lib.pm_collect_rows_grad(self.ctx.h, C.byref(self.desc), T, C.byref(plan), _dev(w), _dev(rows), _dev(dy), _dev(drows),
-                                             _dev(dw)))
+        rc = self.lib.pm_collect_rows_grad(self.ctx.h, self._desc, T, plan, _dev(w), _dev(rows), _dev(dy), _dev(drows), _dev(dw))
+        if rc:
+            _check(rc)
 
 
 class BlockNorm:
@@ -597,26 +604,29 @@ class BlockNorm:
         self.ctx, self.lib = ctx, ctx.lib
         self.desc = NormDesc(STREAM_TYPES[dtype], STREAM_TYPES[wtype], d, PM_NORM_POST * bool(post) | PM_NORM_PRE * bool(pre),
                              NORM_GATES[gate], eps_post, eps_pre, offset_post, offset_pre, alpha, beta, 0, stride, stride, stride, stride)
+        self._desc = C.byref(self.desc)
         self.scratch_bytes(0)
 
     def scratch_bytes(self, T: int) -> int:
         """Bytes of device memory that `grad` of T rows works in."""
-        n = self.lib.pm_block_norm_scratch(self.ctx.h, C.byref(self.desc), T)
+        n = self.lib.pm_block_norm_scratch(self.ctx.h, self._desc, T)
         if n == 0:
             raise PelicaError(-1, self.lib.pm_last_error().decode())
         return n
 
     def forward(self, T: int, x, f, r, n=None, w_post=None, gate=None, w_pre=None):
-        _check(self.lib.pm_block_norm(self.ctx.h, C.byref(self.desc), T, _dev(x), _dev(f), _dev(w_post), _dev(gate), _dev(w_pre), _dev(r),
-                                      _dev(n)))
+        rc = self.lib.pm_block_norm(self.ctx.h, self._desc, T, _dev(x), _dev(f), _dev(w_post), _dev(gate), _dev(w_pre), _dev(r), _dev(n))
+        if rc:
+            _check(rc)
 
     def grad(self, T: int, r, f, dr, dn, dx, df, w_post=None, gate=None, w_pre=None, dw_post=None, dgate=None, dw_pre=None, scratch=None,
              scratch_bytes: int | None = None):
         if scratch_bytes is None:
             scratch_bytes = scratch.nbytes if scratch is not None else 0
-        _check(self.lib.pm_block_norm_grad(self.ctx.h, C.byref(self.desc), T, _dev(r), _dev(f), _dev(w_post), _dev(gate), _dev(w_pre),
-                                           _dev(dr), _dev(dn), _dev(dx), _dev(df), _dev(dw_post), _dev(dgate), _dev(dw_pre), _dev(scratch),
-                                           scratch_bytes))
+        rc = self.lib.pm_block_norm_grad(self.ctx.h, self._desc, T, _dev(r), _dev(f), _dev(w_post), _dev(gate), _dev(w_pre), _dev(dr), _dev(dn),
+                                         _dev(dx), _dev(df), _dev(dw_post), _dev(dgate), _dev(dw_pre), _dev(scratch), scratch_bytes)
+        if rc:
+            _check(rc)
 
 
 class Stack:
