@@ -281,6 +281,14 @@ __global__ void __launch_bounds__(SM / N) k_block_norm(NormCall c, int tpr, int 
     }
     ring.commit();
   };
+  // without a ring a group of 16-byte words has one row: its loads go in front of the weights' (one token 6.2 -> 5.8 us)
+  NormRow<E, V, N> xr, fr;
+  auto fetch = [&](int t) {
+    if (t >= c.T) return;
+    if (has_f) fr.load(c.f, norm_row(t, c.D.f_stride), at, d);
+    if (has_x) xr.load(c.x, norm_row(t, c.D.x_stride), at, d);
+  };
+  if constexpr (!RING && V > 1) fetch(t0);
   ring.clear();
   if constexpr (RING)
     for (int s = 0; s < stages; s++) copy(s, t0 + s * groups);
@@ -293,19 +301,19 @@ __global__ void __launch_bounds__(SM / N) k_block_norm(NormCall c, int tpr, int 
   }
   int turn = 0, stage = 0;
   for (int t = t0; t < c.T; t += groups) {
-    NormRow<E, V, N> xr, fr;
     ring.wait();
-    const uint32_t row = ring.row(stage);
-    if (has_f) ring.get(fr, row, 0, c.f, norm_row(t, c.D.f_stride), at, d);
-    if (has_x) ring.get(xr, row, i_x, c.x, norm_row(t, c.D.x_stride), at, d);
+    if (!RING && (V == 1 || t != t0)) fetch(t);
     if constexpr (RING) {
+      const uint32_t row = ring.row(stage);
+      if (has_f) ring.get(fr, row, 0, c.f, 0, at, d);
+      if (has_x) ring.get(xr, row, i_x, c.x, 0, at, d);
       copy(stage, t + stages * groups);
       stage = stage + 1 == stages ? 0 : stage + 1;
+      wp = ring.slots.template get_vec<N>(0);
     }
-    if constexpr (RING) wp = ring.slots.template get_vec<N>(0);
     VecF<N> r = has_x ? xr.widen() * c.D.alpha : vf_all<N>(0.0f);
+    const VecF<N> f = has_f ? fr.widen() : vf_all<N>(0.0f);
     if (has_f) {
-      const VecF<N> f = fr.widen();
       float s = __fmul_rn(c.D.beta, norm_token_gate<W>(c, t));
       if (post) {
         float sum[1] = {vf_dot(f, f)};
