@@ -2416,14 +2416,16 @@ extern "C" int32_t pm_stack_forward(pm_stack *s, const float *x, int32_t T, floa
     if (!seen) s->seen_T.push_back(T);
     c->ws_off = 0;
   }
-  // residual stream: in place in x_out when it is a device pointer
-  float *xc = is_device_ptr(x_out) ? x_out : ws_take<float>(c, n);
+  // residual stream: in place in x_out when it is a device pointer; of stacks with norms only where it starts on 16 bytes: a layer
+  // without a norm in front of it has the stream itself for its input, which the kernels read 16 bytes at a time
+  const bool x_out_dev = is_device_ptr(x_out), in_place = x_out_dev && (s->norms.empty() || on_16(x_out));
+  float *xc = in_place ? x_out : ws_take<float>(c, n);
   float *xn = ws_take<float>(c, n), *f = s->norms.empty() ? nullptr : ws_take<float>(c, n);
   if (xc != x) CU(cudaMemcpyAsync(xc, x, n * 4, cudaMemcpyDefault, c->stream));
   TRY(stack_layers(s, T, xc, xn, f));
   if (xc != x_out) {
-    CU(cudaMemcpyAsync(x_out, xc, n * 4, cudaMemcpyDeviceToHost, c->stream));
-    CU(cudaStreamSynchronize(c->stream));
+    CU(cudaMemcpyAsync(x_out, xc, n * 4, cudaMemcpyDefault, c->stream));
+    if (!x_out_dev) CU(cudaStreamSynchronize(c->stream));
   }
   return PM_OK;
 }

@@ -116,6 +116,34 @@ def test_refusals_of_stack_norms(tctx):
     layers[0].close()
 
 
+@pytest.mark.parametrize("name", ["c2", "c3", "c4"])
+def test_device_buffers_at_any_start(tctx, name):
+    """x and x_out on the device, in place, one and two values behind 16 bytes: the bits of aligned buffers, also where a layer
+    without a norm in front takes the stream for its input."""
+    cfg = SMALL[name]
+    d = cfg.d
+    layers = layers_of(tctx, cfg, 2)
+    for norms in ([dict(pre=False, post=True)] * 2, [dict(pre=True), dict(pre=False, beta=0.5)], [dict(pre=True, post=True)] * 2):
+        st = pb.Stack(tctx, layers)
+        for i, k in enumerate(norms):
+            st.set_norm(i, *norm_weights(d, i)[:2], **k)
+        for T in (1, 5, 40):
+            x = synth.make_activations(T, d, 60 + T)
+            want = st.forward(x).copy()
+            for shift in (0, 1, 2):
+                src, out = (torch.full((T * d + 8,), 55.0, device="cuda") for _ in range(2))
+                src[shift:shift + T * d] = torch.from_numpy(x).cuda().view(-1)
+                st.set_norm(0, *norm_weights(d, 0)[:2], **norms[0])  # (nothing is recorded any more: the loop runs first)
+                for buf in (out, out, src):  # into another buffer, from a recording where there are few tokens, in place
+                    st.forward_dev(Buf(src[shift:shift + T * d]), T, Buf(buf[shift:shift + T * d]))
+                    tctx.sync()
+                    assert bits_equal(buf[shift:shift + T * d].view(T, d).cpu().numpy(), want), (T, shift)
+                    assert bool((buf[:shift] == 55.0).all()) and bool((buf[shift + T * d:] == 55.0).all())
+        st.close()
+    for layer in layers:
+        layer.close()
+
+
 @pytest.mark.parametrize("name, T", [("c2", 1), ("c2", 37), ("c3", 20), ("c4", 200)])
 def test_the_operators_together(tctx, name, T):
     """norm -> route -> dispatch -> experts on the rows -> collect beside the shared expert -> norm: the layer's own output."""
