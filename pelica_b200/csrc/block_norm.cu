@@ -74,6 +74,15 @@ template <int N> __device__ __forceinline__ float norm_warp_sums(const float (&v
   }
 }
 
+// A CTA may write to another's shared memory only once all of the cluster are known to run: every thread arrives when it begins and
+// waits in front of the first sums, behind the loads of the weights. (Nothing written is handed over: the arrival is relaxed.)
+__device__ __forceinline__ void norm_cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+__device__ __forceinline__ void norm_cluster_wait() {
+  asm volatile("barrier.cluster.wait;" ::: "memory");
+}
+
 // Sums of N values over a row's group, in every thread: lanes, then warps through red (two turns used alternately, so that one
 // barrier a sum is enough), then the cluster's CTAs.
 template <int N> using NormRed = float[2][N == 1 ? 1 : 8][32];
@@ -261,6 +270,7 @@ enum NormMode { NORM_ANY, NORM_SANDWICH, NORM_BEFORE };
 // SM: values of rows that an SM holds
 template <typename E, typename W, int V, int N, int SM, bool CLUSTER, bool RING, NormMode MODE>
 __global__ void __launch_bounds__(SM / N) k_block_norm(NormCall c, int tpr, int rpb, int cl, int stages) {
+  if constexpr (CLUSTER) norm_cluster_arrive();
   pm_pdl();
   extern __shared__ uint4 slots[];
   __shared__ NormRed<1> red;
@@ -299,6 +309,7 @@ __global__ void __launch_bounds__(SM / N) k_block_norm(NormCall c, int tpr, int 
     ring.slots.template put_vec<N>(0, wp);
     ring.slots.template put_vec<N>(N / 4, wn);
   }
+  if constexpr (CLUSTER) norm_cluster_wait();
   int turn = 0, stage = 0;
   for (int t = t0; t < c.T; t += groups) {
     ring.wait();
@@ -340,6 +351,7 @@ __global__ void __launch_bounds__(SM / N) k_block_norm(NormCall c, int tpr, int 
 // its groups and leaves a row of sums in parts[kind][CTA][d], which k_norm_sum_parts adds up. No atomics.
 template <typename E, typename W, int V, int N, int SM, bool CLUSTER, bool RING, NormMode MODE>
 __global__ void __launch_bounds__(SM / N) k_block_norm_grad(NormCall c, int tpr, int rpb, int cl, int stages) {
+  if constexpr (CLUSTER) norm_cluster_arrive();
   pm_pdl();
   extern __shared__ uint4 slots[];
   constexpr int SUMS = MODE == NORM_BEFORE ? 2 : 6;  // r r, u r; f f, dr q, u q, r q
@@ -375,6 +387,7 @@ __global__ void __launch_bounds__(SM / N) k_block_norm_grad(NormCall c, int tpr,
   own.template put_vec<N>(0, norm_weights<W, V, N>(pre ? c.w_pre : nullptr, c.D.offset_pre, at, d));
   own.template put_vec<N>(N / 4, norm_weights<W, V, N>(post ? c.w_post : nullptr, c.D.offset_post, at, d) * norm_weights<W, V, N>(channel ? c.gate : nullptr, 0.0f, at, d));
   VecF<N> a_pre = vf_all<N>(0.0f), a_dk = vf_all<N>(0.0f);
+  if constexpr (CLUSTER) norm_cluster_wait();
   int turn = 0, stage = 0;
   for (int t = t0; t < c.T; t += groups) {
     const size_t at_r = norm_row(t, c.D.r_stride), at_f = norm_row(t, c.D.f_stride), at_n = norm_row(t, c.D.n_stride);
