@@ -565,8 +565,12 @@ class Rows:
         return n
 
     def plan(self, max_rows: int, offset, count, pos, row_pair=None, row_expert=None, row_weight=None) -> RowsPlan:
-        """The buffers of a plan: offset [n_local + 1], count [n_local], pos [T, top_k], the others [max_rows]."""
-        return RowsPlan(*(_dev(p) for p in (offset, count, pos, row_pair, row_expert, row_weight)), max_rows)
+        """The buffers of a plan: offset [n_local + 1], count [n_local], pos [T, top_k], the others [max_rows]. The plan keeps
+        the objects that it is given; behind plain addresses the caller keeps the memory."""
+        buffers = (offset, count, pos, row_pair, row_expert, row_weight)
+        plan = RowsPlan(*(_dev(p) for p in buffers), max_rows)
+        plan.buffers = buffers
+        return plan
 
     def dispatch(self, T: int, ids, plan: RowsPlan, x=None, rows=None, w=None, scale: bool = True):
         """Fills the plan from ids [T, top_k]; rows[pos] = x[t], times w with `scale` and w given."""

@@ -1,5 +1,8 @@
 """What the row and norm operators refuse before they look at a GPU: descriptors, token counts, a missing context."""
 import ctypes as C
+import gc
+import types
+import weakref
 
 import pytest
 
@@ -67,3 +70,21 @@ def test_a_context_and_a_descriptor_are_needed():
     (16384, 16, 512, 0, 256, 262144 + 512 * 255)])
 def test_bound_of_rows(T, top_k, n_exp, n_local, align, want):
     assert LIB.pm_rows_bound(C.byref(pb.RowsDesc(synth.F32, 64, top_k, n_exp, 0, n_local, align)), T) == want
+
+
+def test_a_plan_keeps_its_buffers():
+    """A plan holds addresses for the library: the buffers that it was given live as long as it does."""
+    class Buffer:
+        ptr = 256
+
+    rows = pb.Rows(types.SimpleNamespace(lib=LIB, h=None), 64, 2, 8)
+    buffers = [Buffer() for _ in range(6)]
+    seen = [weakref.ref(b) for b in buffers]
+    plan = rows.plan(64, *buffers)
+    del buffers
+    gc.collect()
+    assert all(r() is not None for r in seen) and plan.pos == 256 and plan.max_rows == 64
+    del plan
+    gc.collect()
+    assert not any(r() is not None for r in seen)
+    assert rows.plan(64, 1, 2, 3).row_pair is None  # (addresses, and none)
