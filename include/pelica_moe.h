@@ -360,7 +360,10 @@ PM_API int32_t pm_quant_act(pm_ctx *ctx, int32_t mode, const float *x, size_t n,
 
 /* ---- tokens sorted by expert and back, and their gradients ------------------
  * No counterpart in the reference: for hosts that run their own products (training, experts of
- * another kind) on the library's routing, and for pm_experts_rows, which wants gathered rows.
+ * another kind) on the library's routing, and for pm_experts_rows, which wants gathered rows: f32, packed
+ * (rows_stride 0), rows 0 .. offset[n_local] - 1 with their row_expert and row_weight, at most
+ * PM_MAX_TOKENS * PM_MAX_TOPK. Where every pair has a row and align is 1 these are T * top_k; else the host reads
+ * offset[n_local] first: what lies behind names no expert.
  * Rows are f32, f16 or bf16; sums are f32, in ascending k, the same bits in every run.
  *
  * All pointers are DEVICE pointers of the context's GPU. The calls allocate nothing, are queued on

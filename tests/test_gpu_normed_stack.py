@@ -181,3 +181,73 @@ def test_the_operators_together(tctx, name, T):
     s = (r.pow(2).mean(1, keepdim=True) + 1e-6).sqrt()
     assert float(((nxt.cpu().double() - r / s) * s).abs().max()) <= 128 * 2.0 ** -24 * 2 * size
     layer.close()
+
+
+@pytest.mark.parametrize("name", ["c2", "c3", "c4"])
+def test_one_layer_against_the_formula(tctx, name):
+    """x <- alpha x + beta gate post(moe(pre(x))) in 64 bits around the layer's own call. Rows of +-2^k without eps have the norm 2^k
+    exactly, so that the layer's input is +-(offset + weight) to the bit and no int8 value of it may round another way; behind the
+    layer the result is off by 40 roundings of 2^-24 of its terms (as the norms alone), and its own."""
+    cfg = SMALL[name]
+    d = cfg.d
+    layers = layers_of(tctx, cfg, 1)
+    st = pb.Stack(tctx, layers)
+    w_pre, w_post, gate = norm_weights(d, 4)
+    for T in (1, 6, 40):
+        rng = np.random.default_rng(T)
+        x = (rng.choice([-1.0, 1.0], (T, d)) * 2.0 ** (np.arange(T) % 5 - 2)[:, None]).astype(np.float32)
+        for pre, post, gated in ((True, True, True), (True, False, False), (False, True, True), (False, False, True)):
+            xn = np.sign(x) * (np.float32(1.0) + w_pre) if pre else x
+            st.set_norm(0, w_pre, w_post, gate if gated else None, pre=pre, post=post, alpha=0.75, beta=1.5, eps_pre=0.0, eps_post=1e-5,
+                        offset_pre=1.0, offset_post=0.5)
+            f = layers[0].forward(xn).astype(np.float64)
+            p = f / np.sqrt((f * f).mean(1, keepdims=True) + 1e-5) * (0.5 + w_post.astype(np.float64)) if post else f
+            a, b = 0.75 * x.astype(np.float64), 1.5 * (gate.astype(np.float64) if gated else 1.0) * p
+            bound = 40 * 2.0 ** -24 * (np.abs(a) + np.abs(b)) + 2.0 ** -24 * np.abs(a + b)
+            buf = torch.from_numpy(x).cuda()
+            for got in (st.forward(x), st.forward(x), st.forward(x)):  # the loop, its recording, a replay
+                assert bool((np.abs(got - (a + b)) <= bound).all()), (T, pre, post, gated)
+            st.forward_dev(Buf(buf), T, Buf(buf))  # in place on the device
+            tctx.sync()
+            assert bits_equal(buf.cpu().numpy(), got)
+    st.close()
+    layers[0].close()
+
+
+@pytest.mark.parametrize("name, T, align", [("c2", 3, 1), ("c2", 70, 16), ("c3", 45, 1), ("c3", 9, 8), ("c4", 150, 4)])
+def test_shards_and_padded_tokens(tctx, name, T, align):
+    """Experts on two ranks and a batch with padded tokens: how many rows a rank has is in offset[n_local], which the host reads;
+    those rows go through pm_experts_rows, and the ranks' shares add up to the layer's pairs. Padded tokens add nothing."""
+    cfg = SMALL[name]
+    W = synth.make_weights(cfg, 3)
+    layer = pb.MoeLayer(tctx, cfg).load(W)
+    d, K, E = cfg.d, cfg.top_k, cfg.n_exp
+    x = synth.make_activations(T, d, 12)
+    ids, w = layer.route(x)
+    pairs = layer.experts_rows(np.repeat(x, K, 0), ids.reshape(-1), w.reshape(-1)).reshape(T, K, d).astype(np.float64)
+    folded = cfg.weight_fold == synth.FOLD_BEFORE_DOWN
+    padded = np.arange(T) % 3 == 1
+    want = (pairs * (1.0 if folded else w.astype(np.float64)[:, :, None])).sum(1)
+    want[padded] = 0.0
+    ids, w = ids.astype(np.uint32), w.copy()
+    ids[padded], w[padded], x[padded] = pb.ROWS_NONE, np.nan, np.inf
+    new = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t, device="cuda")  # noqa: E731
+    x_d, ids_d, w_d, y = torch.from_numpy(x).cuda(), torch.from_numpy(ids.view(np.int32)).cuda(), torch.from_numpy(w).cuda(), new(T, d)
+    for first, n in ((0, E // 2 - 1), (E // 2 - 1, E - E // 2 + 1)):
+        shard = pb.MoeLayer(tctx, cfg.scaled(first_local_expert=first, n_exp_local=n)).load(W)
+        op = pb.Rows(tctx, d, K, E, first_expert=first, n_local=n, align=align)
+        bound = op.bound(T)
+        rows, outs = new(bound, d), new(bound, d)
+        offset, count, pos, expert = (new(*s, t=torch.int32) for s in ((n + 1,), (n,), (T, K), (bound,)))
+        weight = new(bound)
+        plan = op.plan(bound, offset.data_ptr(), count.data_ptr(), pos.data_ptr(), row_expert=expert.data_ptr(), row_weight=weight.data_ptr())
+        op.dispatch(T, ids_d.data_ptr(), plan, x_d.data_ptr(), rows.data_ptr(), w=w_d.data_ptr(), scale=False)
+        tctx.sync()
+        R = int(offset[n])
+        assert 0 < R < bound
+        pb._check(shard.lib.pm_experts_rows(shard.h, rows.data_ptr(), R, expert.data_ptr(), weight.data_ptr(), outs.data_ptr()))
+        op.collect(T, plan, outs.data_ptr(), y.data_ptr(), w=None if folded else w_d.data_ptr(), add=y.data_ptr())
+        tctx.sync()  # (an expert that the shard does not have would be reported here)
+        shard.close()
+    assert tol_ok(y.cpu().numpy(), want) and not y[torch.from_numpy(padded).cuda()].any()
+    layer.close()
