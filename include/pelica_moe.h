@@ -426,8 +426,8 @@ PM_API int32_t pm_collect_rows_grad(pm_ctx *ctx, const pm_rows_desc *desc, int32
  *   p = f / sqrt(mean(f^2) + eps_post) * (offset_post + w_post)   with PM_NORM_POST, else p = f
  *   r = alpha x + beta gate p                                      the stream behind the block
  *   n = r / sqrt(mean(r^2) + eps_pre) * (offset_pre + w_pre)       with PM_NORM_PRE: the next block's input
- * Streams are f32, f16 or bf16, arithmetic is f32 (n comes from r before it is rounded; squares beyond f32 overflow to
- * infinity). Pointers, queueing and recording as for the rows above. */
+ * Streams are f32, f16 or bf16, arithmetic is f32 (n comes from r before it is rounded; squares, and in the gradient products
+ * of two rows' values, overflow to infinity beyond f32). Pointers, queueing and recording as for the rows above. */
 #define PM_NORM_POST 1
 #define PM_NORM_PRE 2
 enum {
@@ -485,7 +485,9 @@ PM_API int32_t pm_stack_decode_kernel_available(pm_stack *stack);
  *   xn = x or, with PM_NORM_PRE, its norm; f = moe(xn); x = alpha x + beta gate p, p = f or, with PM_NORM_POST, its norm.
  * norm: dtype and wtype f32, d the stack's, gate PM_NORM_GATE_NONE or _CHANNEL, strides 0. w_pre, w_post, gate: [d] f32, host or
  * device memory, copied (w_pre, w_post NULL: ones). norm NULL: the plain form (x / rms(x), x += f) again. A stack with norms runs in
- * the general kernels, its steps fused with pm_block_norm's; a failed call leaves the layer as it was. */
+ * the general kernels, its steps fused with pm_block_norm's - one token too, which takes about twice as long as in the plain stack's
+ * one-launch kernel. A failed call leaves the layer as it was. A graph that the host recorded around pm_stack_forward holds the
+ * weights of before: record it again after this call. */
 PM_API int32_t pm_stack_set_norm(pm_stack *stack, int32_t layer, const pm_norm_desc *norm, const float *w_pre,
                                  const float *w_post, const float *gate);
 /* PM_OK, or PM_ERR_TIMEOUT when a device-side wait of an earlier call gave up

@@ -127,7 +127,7 @@ __device__ __forceinline__ float norm_inv(float sum, float inv_d, float eps) {
   return fabsf(e) < 1.0f ? __fmaf_rn(__fmul_rn(0.5f, y), e, y) : y;
 }
 
-// the thread's 8 values of a row as vectors of V: vector j is columns col0 + j * step ...
+// the thread's N values of a row as vectors of V: vector j is columns col0 + j * step ...
 template <typename E, int V, int N> struct NormRow {
   static constexpr int J = N / V;
   Raw<E, V> v[J];

@@ -387,9 +387,10 @@ __global__ void __launch_bounds__(256, rows_ctas(V, KB, SPREAD, DOT))
 
 static uint32_t rows_vectors(const RowsCall &c) { return c.vec ? (uint32_t)c.D.d / (c.D.dtype == PM_TYPE_F32 ? 4 : 8) : (uint32_t)c.D.d; }
 
-// The threads of a token: as many as its row has vectors, but no more than give every SM 32 warps (4096 x 2048 bf16 back to
-// their tokens: 28 us; 8 warps 31, all 30; with dot products, 8192 tokens: 101, 101, 145). Rows that are only written have one
-// read in flight a thread, so they take all (prompt of 4096 x 7168: 101 us, 112 with 32 warps). Where even CTAs of 256
+// The threads of a token: as many as its row has vectors, but doubled only until the launch has 32 warps for every SM (4096 x 2048 bf16
+// back to their tokens: 28 us; 8 warps 31, all 30; with dot products, 8192 tokens: 101, 101, 145). Not all of them are on the
+// SMs at once: the kernels of 16-byte rows with dot products hold 16 warps an SM. Rows that are only written have one read in
+// flight a thread, so they take all (prompt of 4096 x 7168: 101 us, 112 with 32 warps). Where even CTAs of 256
 // threads leave SMs without work, a row without dot products is cut (grid.y).
 template <typename E, int V, int KB, bool SPREAD, bool DOT>
 static cudaError_t rows_go(const Launch &L, const RowsCall &c, const float *w, const void *src, const void *rows, const void *add, void *out,
